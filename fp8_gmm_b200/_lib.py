@@ -75,6 +75,25 @@ class WgradArgs(ctypes.Structure):
     ]
 
 
+class QuantizeRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("in_", c_vp), ("in_ld", c_i64), ("indices", c_vp), ("top_k", ctypes.c_int), ("in_rows", c_i64),
+        ("rows", c_i64), ("cols", c_i64), ("activation", ctypes.c_int), ("codes", c_vp), ("scales", c_fp),
+    ]
+
+
+class Int8GemmArgs(ctypes.Structure):
+    _fields_ = [
+        ("a", c_vp), ("b", c_vp), ("c", c_vp), ("a_scales", c_fp), ("b_scales", c_fp),
+        ("m_sizes", ctypes.POINTER(c_i64)), ("device_m_sizes", c_vp),
+        ("num_groups", ctypes.c_int), ("rows", c_i64), ("n", c_i64), ("k", c_i64),
+    ]
+
+
+class GradDesc(ctypes.Structure):
+    _fields_ = [("in_", c_vp), ("out", c_vp), ("numel", c_i64), ("in_type", ctypes.c_int), ("out_type", ctypes.c_int)]
+
+
 class CopyBlock(ctypes.Structure):
     _fields_ = [("dst", c_vp), ("src", c_vp), ("bytes", ctypes.c_size_t)]
 
@@ -107,6 +126,13 @@ SYMBOLS = {
     "fp8gmm_moe_gather": (ctypes.c_int, [c_vp, c_vp, c_vp, ctypes.c_int, c_i64, c_i64, c_vp, c_vp]),
     "fp8gmm_moe_scatter": (ctypes.c_int, [c_vp, c_vp, c_vp, ctypes.c_int, c_i64, c_i64, c_vp, c_vp]),
     "fp8gmm_moe_rowdot": (ctypes.c_int, [c_vp, c_vp, c_vp, ctypes.c_int, c_i64, c_i64, c_vp, c_vp]),
+    "fp8gmm_quantize_rows_int8": (ctypes.c_int, [ctypes.POINTER(QuantizeRowsArgs), c_vp]),
+    "fp8gmm_int8_grouped_gemm": (ctypes.c_int, [ctypes.POINTER(Int8GemmArgs), c_vp]),
+    "fp8gmm_sum_squares_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int]),
+    "fp8gmm_multi_sum_squares": (ctypes.c_int, [c_vp, ctypes.c_int, c_vp, ctypes.c_size_t, c_vp, c_fp, c_vp]),
+    "fp8gmm_multi_clip": (ctypes.c_int, [c_vp, ctypes.c_int, c_vp, ctypes.c_float, c_fp, c_vp]),
+    "fp8gmm_multi_clip_grad_norm": (
+        ctypes.c_int, [c_vp, ctypes.c_int, ctypes.c_float, c_vp, ctypes.c_size_t, c_fp, c_vp]),
     "fp8gmm_peer_alloc": (ctypes.c_int, [ctypes.c_size_t, ctypes.POINTER(c_vp), c_vp]),
     "fp8gmm_peer_free": (ctypes.c_int, [c_vp]),
     "fp8gmm_peer_open": (ctypes.c_int, [c_vp, ctypes.POINTER(c_vp)]),

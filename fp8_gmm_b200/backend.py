@@ -9,14 +9,17 @@ List-style ops accept any number of tensors per call (the reference stops at 64)
 functions are the allocation-free fast forms the modules use: one base tensor plus host prefix sums
 instead of Python lists of per-group views.
 """
+import contextlib
 import ctypes
+import math
 import os
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import BlockedCastArgs, GemmArgs, GroupedCastArgs, ScaleMulDesc, TensorDesc, WgradArgs, check, lib
+from ._lib import (BlockedCastArgs, GemmArgs, GroupedCastArgs, Int8GemmArgs, QuantizeRowsArgs, ScaleMulDesc, TensorDesc,
+                   WgradArgs, check, lib)
 from .utils import FP8_FORMAT_CODE
 
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
@@ -616,6 +619,233 @@ def grouped_wgrad_rowmajor(dy, x, row_offsets, a_scale_invs, b_scale_invs, c=Non
         check(lib.fp8gmm_grouped_wgrad_rowmajor(ctypes.byref(args), _stream()), "grouped_wgrad_rowmajor")
     del keep
     return c
+
+
+# ------------------------------------------------------------------------------------------------
+# products of 8-bit integers with scales per row and per output channel (evaluation and serving; no counterpart in the
+# reference, which has FP8 only)
+# ------------------------------------------------------------------------------------------------
+def _on(device):
+    """Context in which ``device`` is the current one: the launches below go to the stream of their tensors' device."""
+    if _raw_device is not None and _raw_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _no_grad_wanted(name, *tensors):
+    _require(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)),
+             f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, scales=None):
+    """bf16 rows -> ``(codes, scales)``: int8 codes ``round(127 v / max|v|)`` (ties to even, correctly rounded) and fp32
+    ``scales = max|v| / 127``, one per row ``v``; ``codes * scales`` is the row again.
+
+    x: (..., cols) bf16, rows contiguous.  ``indices`` (CUDA int32, from ``routing.indices_and_bins``): row r is taken
+    from ``x[indices[r] // top_k]``, the gather of an MoE block.  ``activation``: "gelu" (tanh form) or "swiglu" (x is
+    [gate | up], the codes half as wide) is applied first, in fp32.  A row of zeros has scale 0; a row with an infinity
+    or a NaN has codes 0 and scale NaN, so every product of it is NaN.  Weights (G, N, K) give codes of that shape and
+    scales (G, N).  ``codes`` / ``scales``: written in place when given.
+    """
+    _require(x.is_cuda and x.dtype == torch.bfloat16, "quantize_rows_int8: x must be a CUDA bfloat16 tensor")
+    _require(x.dim() >= 2, "quantize_rows_int8: x must have at least two dimensions")
+    _no_grad_wanted("quantize_rows_int8", x)
+    if x.dim() > 2:
+        _require(x.is_contiguous() and indices is None, "quantize_rows_int8: x with more than two dimensions must be contiguous, without indices")
+    else:
+        _require(x.shape[1] <= 1 or x.stride(1) == 1, "quantize_rows_int8: the elements of a row must be contiguous")
+        _require(x.shape[0] <= 1 or x.stride(0) >= x.shape[1], "quantize_rows_int8: the rows of x overlap")
+    _require(activation in (None, "none", "gelu", "swiglu"), f"quantize_rows_int8: unknown activation {activation!r}")
+    width = x.shape[-1]
+    _require(activation != "swiglu" or width % 2 == 0, "quantize_rows_int8: swiglu needs [gate | up] columns")
+    cols = width // 2 if activation == "swiglu" else width
+    if indices is not None:
+        _require(indices.is_cuda and indices.device == x.device and indices.dtype == torch.int32 and indices.dim() == 1
+                 and indices.is_contiguous(), "quantize_rows_int8: indices must be a contiguous 1-D CUDA int32 tensor on the device of x")
+        _require(top_k >= 1, "quantize_rows_int8: top_k must be positive")
+        lead = (indices.numel(),)
+    else:
+        lead = tuple(x.shape[:-1])
+    if codes is None:
+        codes = torch.empty(*lead, cols, dtype=torch.int8, device=x.device)
+    if scales is None:
+        scales = torch.empty(lead, dtype=torch.float32, device=x.device)
+    _require(codes.device == x.device and codes.dtype == torch.int8 and tuple(codes.shape) == lead + (cols,) and codes.is_contiguous(),
+             "quantize_rows_int8: bad codes output")
+    _require(scales.device == x.device and scales.dtype == torch.float32 and tuple(scales.shape) == lead and scales.is_contiguous(),
+             "quantize_rows_int8: bad scales output")
+    args = QuantizeRowsArgs()
+    args.in_, args.in_ld = x.data_ptr(), x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else width
+    args.in_rows = math.prod(x.shape[:-1])
+    args.indices, args.top_k = _ptr(indices), int(top_k)
+    args.rows, args.cols = math.prod(lead), cols
+    args.activation = _ACT_CODE[activation]
+    args.codes, args.scales = codes.data_ptr(), scales.data_ptr()
+    with _on(x.device):
+        check(lib.fp8gmm_quantize_rows_int8(ctypes.byref(args), _stream()), "quantize_rows_int8")
+    return codes, scales
+
+
+def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
+    """Grouped product of int8 codes, ``c[r] = bf16((a[r] . b[g]^T) * a_scales[r] * b_scales[g])`` for the rows r of group g.
+
+    a: (rows, K) int8, b: (G, N, K) int8, a_scales (rows,) and b_scales (G, N) fp32.  The 32-bit integer sums are exact.
+    ``group_sizes``: one size per group, a CPU int64 tensor or a sequence as everywhere in this package (they sum to
+    the rows), or a CUDA int64 tensor that is read when the kernel runs: then nothing waits for the host, the call can
+    be captured into a graph and replayed with other sizes, and rows behind the last group are left as they are.
+    """
+    _require(a.is_cuda and a.dtype == torch.int8 and a.dim() == 2 and a.is_contiguous(), "int8_gmm: a must be a contiguous 2-D CUDA int8 tensor")
+    _require(b.device == a.device and b.dtype == torch.int8 and b.dim() == 3 and b.is_contiguous(),
+             "int8_gmm: b must be a contiguous 3-D int8 tensor on the device of a")
+    rows, k = a.shape
+    G, n = b.shape[0], b.shape[1]
+    _require(b.shape[2] == k, "int8_gmm: contraction dimensions differ")
+    _require(a_scales.device == a.device and a_scales.dtype == torch.float32 and tuple(a_scales.shape) == (rows,) and a_scales.is_contiguous(),
+             "int8_gmm: a_scales must be (rows,) float32 on the device of a")
+    _require(b_scales.device == a.device and b_scales.dtype == torch.float32 and tuple(b_scales.shape) == (G, n) and b_scales.is_contiguous(),
+             "int8_gmm: b_scales must be (G, N) float32 on the device of a")
+    _require(len(group_sizes) == G, "int8_gmm: one group size per expert is required")
+    _no_grad_wanted("int8_gmm", a_scales, b_scales)
+    if c is None:
+        c = torch.empty(rows, n, dtype=torch.bfloat16, device=a.device)
+    _require(c.device == a.device and c.dtype == torch.bfloat16 and tuple(c.shape) == (rows, n) and c.is_contiguous(), "int8_gmm: bad output")
+    args = Int8GemmArgs()
+    keep = None
+    if torch.is_tensor(group_sizes) and group_sizes.is_cuda:
+        _require(group_sizes.device == a.device and group_sizes.dtype == torch.int64 and group_sizes.dim() == 1 and group_sizes.is_contiguous(),
+                 "int8_gmm: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of a")
+        args.device_m_sizes = group_sizes.data_ptr()
+    else:
+        args.m_sizes, keep = _i64_array(group_sizes)
+    args.a, args.b, args.c = a.data_ptr(), b.data_ptr(), c.data_ptr()
+    args.a_scales, args.b_scales = a_scales.data_ptr(), b_scales.data_ptr()
+    args.num_groups, args.rows, args.n, args.k = G, rows, n, k
+    with _on(a.device):
+        check(lib.fp8gmm_int8_grouped_gemm(ctypes.byref(args), _stream()), "int8_gmm")
+    del keep
+    return c
+
+
+def int8_linear(x, weight, group_sizes, weight_scales, indices=None, top_k=1, activation=None, c=None):
+    """bf16 rows through int8 experts: ``quantize_rows_int8`` (with its gather and activation) and ``int8_gmm``.
+
+    x: (rows, K) bf16 sorted by expert, or with ``indices`` the tokens (tokens, K) as the router sees them; weight
+    (G, N, K) int8 with weight_scales (G, N) from ``quantize_rows_int8(weight)``.  Returns (rows, N) bf16, rows sorted by
+    expert."""
+    _require(x.dim() == 2, "int8_linear: x must be a matrix")
+    codes, scales = quantize_rows_int8(x, indices, top_k, activation)
+    return int8_gmm(codes, weight, group_sizes, scales, weight_scales, c)
+
+
+# ------------------------------------------------------------------------------------------------
+# global norm of a list of gradients, and clipping by it (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------------
+_GRAD_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _dense(t):
+    """Whether the elements of t fill one piece of memory, in whatever order of dimensions."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for stride, extent in sorted((s, e) for s, e in zip(t.stride(), t.shape) if e != 1):
+        if stride != size:
+            return False
+        size *= extent
+    return True
+
+
+def _grad_descs(grads, outputs, name):
+    """Descriptor array (fp8gmm_grad_desc: in, out, numel, in_type | out_type << 32) and the common device."""
+    device = grads[0].device
+    rows = []
+    _require(outputs is None or len(outputs) == len(grads), f"{name}: one output per gradient is required")
+    for i, g in enumerate(grads):
+        kind = _GRAD_TYPE.get(g.dtype)
+        _require(kind is not None and g.is_cuda and g.layout == torch.strided, f"{name}: gradient {i} must be a dense CUDA bfloat16, float16 or float32 tensor")
+        _require(g.device == device, f"{name}: gradient {i} is on another device than gradient 0")
+        _require(_dense(g), f"{name}: gradient {i} has gaps or shares elements with itself")
+        if outputs is None:
+            rows += (g.data_ptr(), g.data_ptr(), g.numel(), kind | kind << 32)
+        else:
+            o = outputs[i]
+            out_kind = _GRAD_TYPE.get(o.dtype)
+            _require(out_kind is not None and o.device == device, f"{name}: output {i} must be a bfloat16, float16 or float32 tensor on the device of the gradients")
+            _require(o.shape == g.shape and (o.is_contiguous() and g.is_contiguous() or o.stride() == g.stride()),
+                     f"{name}: output {i} does not have the layout of its gradient")
+            rows += (g.data_ptr(), o.data_ptr(), g.numel(), kind | out_kind << 32)
+    return np.array(rows, dtype=np.int64), device
+
+
+def _grad_workspace(count, device):
+    # taken per call, not kept: a buffer kept per stream would be shared by graphs captured one after the other
+    return torch.empty(lib.fp8gmm_sum_squares_workspace_bytes(count) // 8, dtype=torch.float64, device=device)
+
+
+def multi_sum_squares(grads):
+    """Sum of the squares of all elements as a 0-dim float64 CUDA tensor: the part of a norm that ranks holding shards of
+    the same parameters add up (``all_reduce``) before ``multi_clip``."""
+    grads = list(grads)
+    out = torch.empty((), dtype=torch.float64, device=grads[0].device if grads else "cuda")
+    if not grads:
+        return out.zero_()
+    descs, device = _grad_descs(grads, None, "multi_sum_squares")
+    with _on(device):
+        ws = _grad_workspace(len(grads), device)
+        check(lib.fp8gmm_multi_sum_squares(descs.ctypes.data, len(grads), ws.data_ptr(), ws.numel() * 8, out.data_ptr(), None, _stream()),
+              "multi_sum_squares")
+    return out
+
+
+def multi_grad_norm(grads):
+    """Global 2-norm of a list of CUDA tensors (bfloat16, float16, float32, mixed) as a 0-dim float32 CUDA tensor."""
+    grads = list(grads)
+    out = torch.empty((), dtype=torch.float32, device=grads[0].device if grads else "cuda")
+    if not grads:
+        return out.zero_()
+    descs, device = _grad_descs(grads, None, "multi_grad_norm")
+    with _on(device):
+        ws = _grad_workspace(len(grads), device)
+        check(lib.fp8gmm_multi_sum_squares(descs.ctypes.data, len(grads), ws.data_ptr(), ws.numel() * 8, None, out.data_ptr(), _stream()),
+              "multi_grad_norm")
+    return out
+
+
+def _max_norm(value, name):
+    value = float(value)
+    _require(value >= 0.0, f"{name}: max_norm must be a number that is not negative")
+    return value
+
+
+def multi_clip(grads, sum_squares, max_norm, outputs=None):
+    """Scales every gradient by ``min(1, max_norm / (sqrt(sum_squares) + 1e-6))``, in place or into ``outputs`` (which may
+    have another float type: bf16 gradients into an optimizer's fp32 ones).  ``sum_squares``: 0-dim float64 CUDA tensor
+    (``multi_sum_squares``).  Returns its square root, 0-dim float32; a NaN there makes every output NaN."""
+    grads = list(grads)
+    _require(sum_squares.is_cuda and sum_squares.dtype == torch.float64 and sum_squares.numel() == 1, "multi_clip: sum_squares must be one CUDA float64 value")
+    max_norm = _max_norm(max_norm, "multi_clip")
+    norm = torch.empty((), dtype=torch.float32, device=sum_squares.device)
+    descs, device = _grad_descs(grads, outputs, "multi_clip") if grads else (np.zeros(0, np.int64), sum_squares.device)
+    _require(device == sum_squares.device, "multi_clip: sum_squares is on another device than the gradients")
+    with _on(device):
+        check(lib.fp8gmm_multi_clip(descs.ctypes.data, len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr(), _stream()), "multi_clip")
+    return norm
+
+
+def multi_clip_grad_norm(grads, max_norm, outputs=None):
+    """``multi_grad_norm`` and the clipping of the gradients by it in two launches, without a wait for the host; in place or
+    into ``outputs`` as in ``multi_clip``.  Returns the norm before clipping, 0-dim float32."""
+    grads = list(grads)
+    max_norm = _max_norm(max_norm, "multi_clip_grad_norm")
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device if grads else "cuda")
+    if not grads:
+        return norm.zero_()
+    descs, device = _grad_descs(grads, outputs, "multi_clip_grad_norm")
+    with _on(device):
+        ws = _grad_workspace(len(grads), device)
+        check(lib.fp8gmm_multi_clip_grad_norm(descs.ctypes.data, len(grads), max_norm, ws.data_ptr(), ws.numel() * 8, norm.data_ptr(), _stream()),
+              "multi_clip_grad_norm")
+    return norm
 
 
 def delayed_scaling_update(amax_history, scale, scale_inv, fp8_max, margin=0, algo="max"):

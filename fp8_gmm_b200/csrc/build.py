@@ -24,6 +24,9 @@ SOURCES = [
     ("runtime.cu", []),
     ("peer.cu", []),
     ("routing.cu", []),
+    ("grad_norm.cu", []),
+    ("int8_quantize.cu", []),
+    ("int8_gemm.cu", []),
     ("pointwise.cu", ["--use_fast_math"]),
     ("pad_fusion.cu", ["--use_fast_math"]),
     ("gemm_sm100.cu", ["--use_fast_math"]),

@@ -400,6 +400,95 @@ int fp8gmm_moe_rowdot(const void* grad, const void* x, const int32_t* inverse, i
                       float* d_weights, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Products of 8-bit integers with a scale for each row (token) and each output channel: evaluation and serving of the
+ * experts without the amax history that delayed scaling needs.  No counterpart in the reference (FP8 only).
+ * ---------------------------------------------------------------------------------------------- */
+
+/*
+ * Rows of bf16 -> int8 codes and one fp32 scale per row:
+ *   v = act(in[src(r), :]), top = max|v|, scales[r] = top / 127, codes[r, k] = round_half_even(127 * v[k] / top)
+ * with src(r) = r, or indices[r] / top_k (the permutation fp8gmm_moe_sort writes: the gather of an MoE block, fused).
+ * activation: FP8GMM_ACT_NONE, _GELU (tanh form), or _SWIGLU (a row of `in` is then [gate | up], 2 * cols wide).
+ * A row of zeros gets scale 0; a row with an infinity or a NaN gets codes 0 and scale NaN.  An index that names no row of
+ * `in` gives codes 0 and scale 0 and is reported through the device status word.
+ * Weights (G x N x K) are quantised per output channel by the same call, as G * N rows of K columns.
+ */
+typedef struct {
+  const void* in;         /* bf16, row pitch in_ld elements (elements of a row are contiguous) */
+  int64_t in_ld;
+  const int32_t* indices; /* device int32[rows], or NULL */
+  int top_k;              /* with indices */
+  int64_t in_rows;        /* rows of `in`; without indices equal to rows */
+  int64_t rows;
+  int64_t cols;           /* columns of codes */
+  int activation;
+  void* codes;            /* int8 (rows x cols) row-major */
+  float* scales;          /* fp32[rows] */
+} fp8gmm_quantize_rows_args;
+
+int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* args, void* stream);
+
+/*
+ * C[r, :] = bf16( (sum_k a[r, k] * b[g, :, k]) * a_scales[r] * b_scales[g, :] ) for every row r of group g; 32-bit integer
+ * sums (exact: K < 131072).
+ *   a        int8 (rows x K) row-major, groups are consecutive row blocks
+ *   b        int8 (G x N x K) row-major
+ *   c        bf16 (rows x N)
+ *   m_sizes  HOST int64[num_groups], sum = rows; or NULL and
+ *   device_m_sizes  DEVICE int64[num_groups], read when the kernel runs (a router's histogram, without a round trip to the
+ *            host; the call can then be captured into a graph and replayed with other sizes).  Rows behind the last group
+ *            are neither read nor written.  Sizes that are negative or reach behind `rows` are cut off and reported
+ *            through the device status word.
+ * N and K must be multiples of 16, num_groups <= 512, pointers 16-byte aligned.
+ */
+typedef struct {
+  const void* a;
+  const void* b;
+  void* c;
+  const float* a_scales;
+  const float* b_scales;
+  const int64_t* m_sizes;
+  const int64_t* device_m_sizes;
+  int num_groups;
+  int64_t rows;
+  int64_t n;
+  int64_t k;
+} fp8gmm_int8_gemm_args;
+
+int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Global 2-norm of a list of gradients, and clipping by it: what stands between the weight gradients and the optimizer.
+ * No counterpart in the reference.  Any number of tensors of mixed types per call; the sum is kept in double precision and
+ * added up in a fixed order (the same bits on every run).
+ * ---------------------------------------------------------------------------------------------- */
+typedef enum { FP8GMM_BF16 = 0, FP8GMM_F16 = 1, FP8GMM_F32 = 2 } fp8gmm_type;
+
+typedef struct {
+  const void* in; /* contiguous elements */
+  void* out;      /* clipped elements; the same array as `in` clips in place; ignored by fp8gmm_multi_sum_squares */
+  int64_t numel;
+  int in_type;    /* fp8gmm_type */
+  int out_type;
+} fp8gmm_grad_desc;
+
+size_t fp8gmm_sum_squares_workspace_bytes(int count);
+
+/* *sum = sum of squares of all elements (double), *norm = its square root (float); device pointers, either may be NULL.
+ * `workspace`: device memory, 8-byte aligned, free again once the call's work has run.  An empty list gives 0. */
+int fp8gmm_multi_sum_squares(const fp8gmm_grad_desc* descs, int count, void* workspace, size_t workspace_bytes, double* sum,
+                             float* norm, void* stream);
+
+/* out = in * min(1, max_norm / (sqrt(*sum) + 1e-6)) for a sum of squares on the device, for instance one that was added up
+ * over the ranks that hold the parameters' shards.  *norm = sqrt(*sum) unless NULL.  A NaN norm makes every output NaN.
+ * Entries that write an element another entry reads or writes are refused. */
+int fp8gmm_multi_clip(const fp8gmm_grad_desc* descs, int count, const double* sum, float max_norm, float* norm, void* stream);
+
+/* Both in one call. */
+int fp8gmm_multi_clip_grad_norm(const fp8gmm_grad_desc* descs, int count, float max_norm, void* workspace, size_t workspace_bytes,
+                                float* norm, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Peer-memory transport for the expert-parallel row exchange (dispatch / combine between the GPUs of one
  * NVSwitch node).  No counterpart in the reference, which is single-GPU apart from one all-reduce
  * (reference fp8_gmm/grouped_mlp.py:300-303) and permutes rows on one device (fp8_gmm/example.py:52-59).

@@ -1,0 +1,347 @@
+"""GPU: int8 row quantisation and grouped product against the definition in 64 bits.
+
+The codes and the integer sums are exact, so without an activation every output is compared bit for bit: codes with the
+correctly rounded quotient, products with fp32(sum) * fp32(scale * scale) rounded to bf16, which fp32 torch on the CPU
+reproduces.  Behind an activation the row is known to the accuracy of fp32's exp and division (relative error below 2^-17,
+dominated by the argument of exp: |x| log2(e) 2^-24 at |x| <= 80), which moves a quotient of at most 127 by less than
+127 * 2 * 2^-17 = 0.002."""
+import pytest
+import torch
+
+from tests.helpers import randn_bf16, routed_group_sizes
+
+pytestmark = pytest.mark.gpu
+ACT_REL = 2.0 ** -17
+
+
+def _act64(x, act):
+    v = x.double()
+    if act == "swiglu":
+        g, u = v.chunk(2, dim=-1)
+        return g / (1 + torch.exp(-g)) * u
+    if act == "gelu":
+        return v / (1 + torch.exp(-2 * 0.79788456 * v * (1 + 0.044715 * v * v)))
+    return v
+
+
+def _quantize64(x):
+    """(codes, scales) of rows without an activation: quotients in 64 bits, the scale as one fp32 division."""
+    v = x.double()
+    top = v.abs().amax(-1, keepdim=True)
+    q = torch.round(v * 127 / torch.where(top > 0, top, torch.ones_like(top)))
+    return q.to(torch.int8), top[..., 0].float() / 127
+
+
+def _product(a, b, sizes, sa, sb):
+    """int64 sums, then the kernel's three fp32 roundings and the bf16 one."""
+    out, r = [], 0
+    for g, m in enumerate(sizes):
+        acc = (a[r:r + m].double() @ b[g].double().t())    # exact: below 2^53
+        out.append((acc.float() * (sa[r:r + m, None] * sb[g][None])).to(torch.bfloat16))
+        r += m
+    return torch.cat(out) if out else torch.empty(0, b.shape[1], dtype=torch.bfloat16)
+
+
+def _codes(shape, seed, lo=-127, hi=127):
+    return torch.randint(lo, hi + 1, shape, generator=torch.Generator().manual_seed(seed), dtype=torch.int32).to(torch.int8)
+
+
+def _scales(shape, seed):
+    return torch.rand(shape, generator=torch.Generator().manual_seed(seed)) * 0.01 + 1e-4
+
+
+# ------------------------------------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 16), (2, 33), (7, 677), (1, 1481), (33, 4096), (2, 14336), (4, 40961), (300, 128), (2, 131056)])
+def test_codes_are_correctly_rounded(cuda, rows, cols):
+    from fp8_gmm_b200 import backend
+
+    x = randn_bf16((rows, cols), rows * 7 + cols, std=3.0)
+    q, s = backend.quantize_rows_int8(x.to(cuda))
+    want_q, want_s = _quantize64(x)
+    assert q.shape == (rows, cols) and torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+
+
+def test_ties_extremes_and_special_rows(cuda):
+    """Half-way quotients (top * (2 i + 1) / 254 is representable for top = 127 * 2^e), the type's extremes, rows of zeros,
+    rows with infinities or NaN."""
+    from fp8_gmm_b200 import backend
+
+    ties = (torch.arange(-127, 127) + 0.5)
+    inf, nan = float("inf"), float("nan")
+    rows = [torch.cat([torch.tensor([127.0]), ties]) * 2.0 ** e for e in (0, 20, -40, 110, -120)]
+    rows += [torch.cat([torch.tensor([1.0, 0.5, -0.5, 0.25]), torch.linspace(-1, 1, 251)]) * f for f in (1.0, 1.7, 3e38, 1e-38)]
+    rows += [torch.zeros(255), torch.full((255,), -0.0), torch.full((255,), 9.2e-41), torch.full((255,), 3.3895e38)]
+    x = torch.stack(rows).to(torch.bfloat16)
+    q, s = backend.quantize_rows_int8(x.to(cuda))
+    want_q, want_s = _quantize64(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+    bad = torch.ones(4, 255, dtype=torch.bfloat16)
+    bad[0, 17], bad[1, 254], bad[2, 0] = inf, nan, -inf
+    q, s = backend.quantize_rows_int8(bad.to(cuda))
+    assert (q[:3] == 0).all() and s[:3].isnan().all() and (q[3] == 127).all() and float(s[3]) == float(torch.tensor(1.0) / 127)
+
+
+@pytest.mark.parametrize("act", ["gelu", "swiglu"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 33), (3, 1024), (2, 14336), (65, 272)])
+def test_activation_in_front(cuda, act, rows, cols):
+    from fp8_gmm_b200 import backend
+
+    x = randn_bf16((rows, cols * (2 if act == "swiglu" else 1)), rows + cols, std=4.0)
+    q, s = backend.quantize_rows_int8(x.to(cuda), activation=act)
+    v = _act64(x, act)
+    top = v.abs().amax(1, keepdim=True)
+    assert torch.allclose(s.cpu().double(), top[:, 0] / 127, rtol=ACT_REL + 2.0 ** -23, atol=0)
+    assert float((q.cpu().double() - v * 127 / top).abs().max()) <= 0.5 + 127 * 2 * ACT_REL
+
+
+def test_activation_far_out(cuda):
+    """Gates where exp overflows: the activation is 0 or the identity, never NaN."""
+    from fp8_gmm_b200 import backend
+
+    x = torch.tensor([[-1e4, 1e4, -200.0, 90.0, 0.0, -1e30, 2.0, 2.0, 2.0, 2.0, 2.0, 2.0]]).to(torch.bfloat16)
+    q, s = backend.quantize_rows_int8(x.to(cuda), activation="swiglu")
+    assert q.cpu().tolist() == [[0, 127, 0, 1, 0, 0]] and torch.isfinite(s).all()
+    q, s = backend.quantize_rows_int8(x.to(cuda)[:, :5].contiguous(), activation="gelu")
+    assert q.cpu().tolist() == [[0, 127, 0, 1, 0]] and torch.isfinite(s).all()
+
+
+def test_rows_with_a_pitch_an_offset_and_three_dimensions(cuda):
+    from fp8_gmm_b200 import backend
+
+    base = randn_bf16((9, 200), 1).to(cuda)
+    for view in (base[:, :64], base[:, 8:72], base[:, 1:66], base[::2, 3:4], base[1:2, 5:105]):
+        q, s = backend.quantize_rows_int8(view)
+        want_q, want_s = _quantize64(view.cpu())
+        assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+    w = randn_bf16((3, 16, 48), 2)
+    q, s = backend.quantize_rows_int8(w.to(cuda))
+    want_q, want_s = _quantize64(w)
+    assert q.shape == w.shape and s.shape == (3, 16) and torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+    codes, scales = torch.empty_like(q), torch.empty_like(s)
+    got = backend.quantize_rows_int8(w.to(cuda), codes=codes, scales=scales)
+    assert got[0] is codes and torch.equal(codes, q) and torch.equal(scales, s)
+
+
+def test_gather_by_indices(cuda):
+    from fp8_gmm_b200 import _lib, backend
+
+    x = randn_bf16((11, 136), 3)
+    idx = torch.tensor([0, 0, 21, 5, 7, 20, 20, 13], dtype=torch.int32)    # the same row several times
+    q, s = backend.quantize_rows_int8(x.to(cuda), idx.to(cuda), 2)
+    want_q, want_s = _quantize64(x[idx.long() // 2])
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+    backend.device_status()
+    idx[3], idx[5] = -1, 22                                                # name no row: zeros, reported
+    q, s = backend.quantize_rows_int8(x.to(cuda), idx.to(cuda), 2)
+    assert _lib.lib.fp8gmm_device_status(torch.cuda.current_stream().cuda_stream) == 4
+    for r in (3, 5):
+        assert (q[r] == 0).all() and float(s[r]) == 0.0
+    keep = [0, 1, 2, 4, 6, 7]
+    assert torch.equal(q.cpu()[keep], want_q[keep])
+    q, s = backend.quantize_rows_int8(x.to(cuda), idx[:0].to(cuda), 2)
+    assert q.shape == (0, 136) and s.shape == (0,)
+
+
+# ------------------------------------------------------------------------------------------------ product
+@pytest.mark.parametrize("sizes,n,k", [
+    ([1], 16, 16), ([0, 1, 0], 16, 48), ([3], 128, 128), ([2, 0, 5], 272, 144), ([16, 17, 0, 1], 144, 272), ([31, 33], 1424, 2080),
+    ([64, 65, 0, 1, 127], 48, 4112), ([300, 0, 24, 17], 512, 768), ([128, 128], 256, 256), ([129, 255, 257], 400, 64), ([513], 1040, 1024),
+    ([1] * 37, 64, 112), ([700, 3, 900], 528, 176), ([0, 0], 32, 32), ([2], 4096, 14336), ([1, 1], 16, 131056),
+])
+def test_product_is_exact(cuda, sizes, n, k):
+    from fp8_gmm_b200 import backend
+
+    rows, G = sum(sizes), len(sizes)
+    a, b = _codes((rows, k), 1, -128), _codes((G, n, k), 2, -128)
+    sa, sb = _scales((rows,), 3), _scales((G, n), 4)
+    want = _product(a, b, sizes, sa, sb)
+    dev = [t.to(cuda) for t in (a, b, sa, sb)]
+    got = backend.int8_gmm(dev[0], dev[1], torch.tensor(sizes), dev[2], dev[3])
+    assert torch.equal(got.cpu(), want)
+    on_gpu = backend.int8_gmm(dev[0], dev[1], torch.tensor(sizes, device=cuda), dev[2], dev[3])
+    backend.device_status()
+    assert torch.equal(on_gpu, got)
+
+
+def test_largest_sums_do_not_overflow(cuda):
+    from fp8_gmm_b200 import backend
+
+    k = 131056
+    a, b = torch.full((2, k), -128, dtype=torch.int8), torch.full((1, 16, k), -128, dtype=torch.int8)
+    b[0, 1] = 127
+    one = torch.ones(2)
+    got = backend.int8_gmm(a.to(cuda), b.to(cuda), [2], one.to(cuda), torch.ones(1, 16).to(cuda))
+    assert torch.equal(got.cpu(), _product(a, b, [2], one, torch.ones(1, 16)))
+
+
+def test_many_rows_in_few_and_many_groups(cuda):
+    """Row counts around every tile size of the kernel, compared on the GPU in 64 bits."""
+    from fp8_gmm_b200 import backend
+
+    n, k = 272, 320
+    for G, rows, seed in [(1, 4097, 1), (3, 5000, 2), (64, 6144, 3), (200, 3000, 4), (512, 700, 5)]:
+        sizes = routed_group_sizes(G, rows, seed)
+        a, b = _codes((rows, k), seed).to(cuda), _codes((G, n, k), seed + 9).to(cuda)
+        sa, sb = _scales((rows,), 3).to(cuda), _scales((G, n), 4).to(cuda)
+        got = backend.int8_gmm(a, b, sizes, sa, sb)
+        assert torch.equal(got, _product(a, b, sizes, sa, sb))
+
+
+def test_sizes_on_the_gpu_leave_the_rows_behind_alone(cuda):
+    from fp8_gmm_b200 import _lib, backend
+
+    a, b = _codes((50, 64), 1).to(cuda), _codes((3, 48, 64), 2).to(cuda)
+    sa, sb = _scales((50,), 3).to(cuda), _scales((3, 48), 4).to(cuda)
+    for sizes in ([10, 0, 23], [0, 0, 0], [50, 0, 0]):
+        c = torch.full((50, 48), 7.0, dtype=torch.bfloat16, device=cuda)
+        backend.int8_gmm(a, b, torch.tensor(sizes, device=cuda), sa, sb, c=c)
+        backend.device_status()
+        m = sum(sizes)
+        assert torch.equal(c[:m].cpu(), _product(a.cpu(), b.cpu(), sizes, sa.cpu(), sb.cpu())) and (c[m:] == 7.0).all()
+    # sizes that do not fit are cut off and reported
+    for sizes, cut in ([20, 40, 5], [20, 30, 0]), ([-3, 20, 1 << 40], [0, 20, 30]):
+        c = torch.full((50, 48), 7.0, dtype=torch.bfloat16, device=cuda)
+        backend.int8_gmm(a, b, torch.tensor(sizes, device=cuda), sa, sb, c=c)
+        assert _lib.lib.fp8gmm_device_status(torch.cuda.current_stream().cuda_stream) == 4
+        assert torch.equal(c.cpu(), _product(a.cpu(), b.cpu(), cut, sa.cpu(), sb.cpu()))
+
+
+def test_a_bad_row_spoils_no_other(cuda):
+    from fp8_gmm_b200 import backend
+
+    x = randn_bf16((6, 64), 1)
+    w = _codes((2, 32, 64), 2).to(cuda)
+    ws = _scales((2, 32), 3).to(cuda)
+    good = backend.int8_linear(x.to(cuda), w, [4, 2], ws)
+    x[1, 5], x[5, 0] = float("nan"), float("inf")
+    got = backend.int8_linear(x.to(cuda), w, [4, 2], ws)
+    assert got[[1, 5]].isnan().all() and torch.equal(got[[0, 2, 3, 4]], good[[0, 2, 3, 4]])
+    x[:] = 0
+    assert (backend.int8_linear(x.to(cuda), w, [4, 2], ws) == 0).all()
+
+
+def test_refusals_on_the_gpu(cuda):
+    from fp8_gmm_b200 import backend
+
+    x, w, ws = torch.zeros(4, 32, dtype=torch.bfloat16, device=cuda), torch.zeros(2, 16, 32, dtype=torch.int8, device=cuda), torch.zeros(2, 16, device=cuda)
+    wide = torch.zeros(2, 32, dtype=torch.bfloat16, device=cuda)
+    bad = [
+        (lambda: backend.int8_linear(x, w, [2, 3], ws), "sum|bad size"), (lambda: backend.int8_linear(x, w, [4], ws), "group size"),
+        (lambda: backend.int8_linear(x, w, torch.tensor([2, 2], dtype=torch.int32, device=cuda), ws), "int64"),
+        (lambda: backend.int8_linear(x[:, ::2], w, [2, 2], ws), "contiguous"), (lambda: backend.int8_linear(x.float(), w, [2, 2], ws), "bfloat16"),
+        (lambda: backend.int8_linear(x, w.float(), [2, 2], ws), "int8"), (lambda: backend.int8_linear(x, w, [2, 2], ws.half()), "float32"),
+        (lambda: backend.int8_linear(x, w[:, :, :16].contiguous(), [2, 2], ws), "contraction"),
+        (lambda: backend.int8_linear(x, w, [2, 2], ws, activation="relu"), "activation"),
+        (lambda: backend.int8_linear(x, w, [2, 2], ws, c=wide), "output"),
+        (lambda: backend.quantize_rows_int8(x, torch.zeros(4, dtype=torch.int64, device=cuda)), "int32"),
+        (lambda: backend.quantize_rows_int8(x.expand(4, 32)[0:1].expand(4, 32)), "overlap"),
+        (lambda: backend.quantize_rows_int8(x[:, :31].contiguous(), activation="swiglu"), "gate"),
+        (lambda: backend.int8_linear(x.clone().requires_grad_(True), w, [2, 2], ws), "no gradient"),
+    ]
+    for call, message in bad:
+        with pytest.raises(RuntimeError, match=message):
+            call()
+
+
+# ------------------------------------------------------------------------------------------------ modules, streams, graphs
+def _moe(experts, gate, tokens, E, top_k):
+    from fp8_gmm_b200 import routing
+
+    weights, selected = routing.topk(tokens @ gate, top_k)
+    indices, bin_ids, bins, sizes = routing.indices_and_bins(selected, E)
+    rows = experts(tokens, sizes, indices=indices, top_k=top_k)
+    return routing.scatter(rows, indices, bin_ids, weights, bins, top_k)
+
+
+@pytest.mark.parametrize("activation", ["gelu", "swiglu"])
+def test_experts_behind_the_router(cuda, activation):
+    """Int8GroupedMlp behind topk -> sort -> scatter equals the same experts evaluated one by one with sizes on the host;
+    against the bf16 weights in 64 bits its error is that of 8-bit rounding (each operand off by at most half a code step:
+    relative error per product about 1 / 127 / sqrt(12) * (top / rms), summed over two layers: below 5 % here)."""
+    import fp8_gmm_b200 as fg
+    from fp8_gmm_b200 import backend, routing
+
+    E, top_k, H, F, T = 6, 2, 256, 272, 97
+    torch.manual_seed(0)
+    mlp = fg.GroupedMlp(H, F, E, torch.bfloat16, device=cuda, activation=activation)
+    experts = fg.Int8GroupedMlp.from_mlp(mlp)
+    tokens, gate = randn_bf16((T, H), 1).to(cuda), randn_bf16((H, E), 2).to(cuda)
+    with torch.no_grad():
+        out = _moe(experts, gate, tokens, E, top_k)
+        weights, selected = routing.topk(tokens @ gate, top_k)
+        indices, bin_ids, bins, sizes = routing.indices_and_bins(selected, E)
+        rows = routing.gather(tokens, indices, bin_ids, bins, top_k)
+        on_host = experts(rows, sizes.cpu())
+        assert torch.equal(routing.scatter(on_host, indices, bin_ids, weights, bins, top_k), out)
+        parts = rows.double().split(sizes.tolist())
+        want = torch.cat([_act64(p @ mlp.fc1_weight[g].double().t(), activation) @ mlp.fc2_weight[g].double().t() for g, p in enumerate(parts)])
+        assert float((on_host.double() - want).norm() / want.norm()) < 0.05
+        lin = fg.GroupedLinear(H, 48, E, torch.bfloat16, device=cuda)
+        q = fg.Int8GroupedLinear.from_linear(lin)
+        got = q(tokens, sizes, indices=indices, top_k=top_k)
+        assert torch.equal(got, backend.int8_linear(rows, q.weight, sizes.cpu(), q.weight_scales))
+    backend.device_status()
+
+
+def test_module_state_round_trip(cuda):
+    import fp8_gmm_b200 as fg
+
+    mlp = fg.GroupedMlp(64, 96, 3, torch.bfloat16, device=cuda, activation="swiglu")
+    a = fg.Int8GroupedMlp.from_mlp(mlp)
+    b = fg.Int8GroupedMlp(64, 96, 3, device=cuda, activation="swiglu")
+    b.load_state_dict(a.state_dict())
+    x = randn_bf16((10, 64), 5).to(cuda)
+    assert torch.equal(a(x, [3, 0, 7]), b(x, [3, 0, 7]))
+
+
+def test_captured_experts_follow_new_tokens_routes_and_weights(cuda):
+    import fp8_gmm_b200 as fg
+
+    E, top_k, H, F, T = 8, 2, 128, 144, 13
+    torch.manual_seed(1)
+    mlp = fg.GroupedMlp(H, F, E, torch.bfloat16, device=cuda, activation="swiglu")
+    experts = fg.Int8GroupedMlp.from_mlp(mlp)
+    tokens, gate = randn_bf16((T, H), 1).to(cuda), randn_bf16((H, E), 2).to(cuda)
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _moe(experts, gate, tokens, E, top_k)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs, outs = [], []
+        for _ in range(2):     # two graphs of the same layer, replayed at the same time on two streams
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(_moe(experts, gate, tokens, E, top_k))
+            graphs.append(g)
+        for seed in (3, 4):
+            tokens.copy_(randn_bf16((T, H), seed))
+            mlp.fc1_weight.mul_(1.01 if seed == 4 else 1.0)
+            experts.refresh(mlp)
+            torch.cuda.synchronize()
+            streams = [torch.cuda.Stream() for _ in graphs]
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    for _ in range(5):
+                        g.replay()
+            torch.cuda.synchronize()
+            want = _moe(experts, gate, tokens, E, top_k)
+            assert all(torch.equal(o, want) for o in outs)
+    fg.backend.device_status()
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    from fp8_gmm_b200 import backend
+
+    w, ws = _codes((4, 272, 512), 2).to(cuda), _scales((4, 272), 3).to(cuda)
+    xs = [randn_bf16((m, 512), m).to(cuda) for m in (5, 333)]
+    sizes = [[1, 0, 2, 2], [100, 33, 0, 200]]
+    want = [backend.int8_linear(x, w, m, ws) for x, m in zip(xs, sizes)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(backend.int8_linear(xs[i], w, sizes[i], ws))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
