@@ -75,6 +75,12 @@ def set_gemm_variant(ctas=0, tail_split=True, tma_epilogue=True):
     check(lib.fp8gmm_set_gemm_variant(int(ctas), int(bool(tail_split)), int(bool(tma_epilogue))), "set_gemm_variant")
 
 
+def set_int8_variant(tile_rows=0, splits=0):
+    """Force the tile of the int8 product (rows of a tile: 16, 32, 64, 128 or 256; CTAs that share its contraction: 1, 2, 4 or
+    8; 0 = automatic); see fp8gmm_set_int8_variant.  For tests and experiments: results are bit-identical."""
+    check(lib.fp8gmm_set_int8_variant(int(tile_rows), int(splits)), "set_int8_variant")
+
+
 def set_wait_limits(gemm_wait_s=0.0, peer_wait_s=0.0):
     """Limits of the kernels' bounded waits in seconds (0 keeps the current value); see fp8gmm_set_wait_limits."""
     check(lib.fp8gmm_set_wait_limits(int(gemm_wait_s * 1e9), int(peer_wait_s * 1e9)), "set_wait_limits")

@@ -457,6 +457,11 @@ typedef struct {
 
 int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
 
+/* Process-wide switch of the launches above, for tests and experiments: rows of a tile (16, 32, 64, 128, or 256 = CTA pairs;
+ * 0 = chosen per call, the default) and the CTAs that share the contraction of a tile of at most 128 rows (1, 2, 4, 8; 0 =
+ * chosen per call).  Results are bit-identical. */
+int fp8gmm_set_int8_variant(int tile_rows, int splits);
+
 /* ------------------------------------------------------------------------------------------------
  * Global 2-norm of a list of gradients, and clipping by it: what stands between the weight gradients and the optimizer.
  * No counterpart in the reference.  Any number of tensors of mixed types per call; the sum is kept in double precision and

@@ -163,6 +163,31 @@ def test_product_is_exact(cuda, sizes, n, k):
     assert torch.equal(on_gpu, got)
 
 
+@pytest.fixture
+def any_variant():
+    from fp8_gmm_b200 import backend
+
+    yield backend.set_int8_variant
+    backend.set_int8_variant()
+
+
+@pytest.mark.parametrize("tile_rows,splits", [(16, 1), (16, 2), (16, 4), (16, 8), (32, 1), (32, 8), (64, 1), (64, 4), (128, 1), (128, 8), (256, 0)])
+def test_every_tile_and_split_gives_the_same_bits(cuda, any_variant, tile_rows, splits):
+    from fp8_gmm_b200 import backend
+
+    any_variant(tile_rows, splits)
+    for sizes, n, k in [([1], 16, 16), ([5, 0, 16, 17, 33], 272, 1040), ([64, 129, 1, 255, 256, 257], 400, 2080), ([2, 7], 1424, 4112), ([300], 128, 128)]:
+        rows, G = sum(sizes), len(sizes)
+        a, b = _codes((rows, k), 1, -128), _codes((G, n, k), 2, -128)
+        sa, sb = _scales((rows,), 3), _scales((G, n), 4)
+        want = _product(a, b, sizes, sa, sb)
+        c = torch.full((rows + 3, n), 7.0, dtype=torch.bfloat16, device=cuda)
+        for m in (torch.tensor(sizes), torch.tensor(sizes, device=cuda)):
+            backend.int8_gmm(a.to(cuda), b.to(cuda), m, sa.to(cuda), sb.to(cuda), c=c[:rows])
+            backend.device_status()
+            assert torch.equal(c[:rows].cpu(), want) and (c[rows:] == 7.0).all()
+
+
 def test_largest_sums_do_not_overflow(cuda):
     from fp8_gmm_b200 import backend
 
