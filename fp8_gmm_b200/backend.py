@@ -643,6 +643,36 @@ def _no_grad_wanted(name, *tensors):
              f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
+def _quantize_args(x, indices, top_k, activation):
+    """Checked arguments of the row quantisation without its outputs, and the leading shape of those."""
+    _require(x.is_cuda and x.dtype == torch.bfloat16, "quantize_rows_int8: x must be a CUDA bfloat16 tensor")
+    dim, shape = x.dim(), x.shape
+    _require(dim >= 2, "quantize_rows_int8: x must have at least two dimensions")
+    _no_grad_wanted("quantize_rows_int8", x)
+    if dim > 2:
+        _require(x.is_contiguous() and indices is None, "quantize_rows_int8: x with more than two dimensions must be contiguous, without indices")
+    else:
+        _require(shape[1] <= 1 or x.stride(1) == 1, "quantize_rows_int8: the elements of a row must be contiguous")
+        _require(shape[0] <= 1 or x.stride(0) >= shape[1], "quantize_rows_int8: the rows of x overlap")
+    _require(activation in (None, "none", "gelu", "swiglu"), f"quantize_rows_int8: unknown activation {activation!r}")
+    width = shape[-1]
+    _require(activation != "swiglu" or width % 2 == 0, "quantize_rows_int8: swiglu needs [gate | up] columns")
+    args = QuantizeRowsArgs()
+    if indices is not None:
+        _require(indices.is_cuda and indices.device == x.device and indices.dtype == torch.int32 and indices.dim() == 1
+                 and indices.is_contiguous(), "quantize_rows_int8: indices must be a contiguous 1-D CUDA int32 tensor on the device of x")
+        _require(top_k >= 1, "quantize_rows_int8: top_k must be positive")
+        args.indices, args.top_k = indices.data_ptr(), int(top_k)
+        lead = tuple(indices.shape)
+    else:
+        lead = tuple(shape[:-1])
+    args.in_, args.in_ld = x.data_ptr(), x.stride(0) if dim == 2 and shape[0] > 1 else width
+    args.in_rows, args.rows = math.prod(shape[:-1]), math.prod(lead)
+    args.cols = width // 2 if activation == "swiglu" else width
+    args.activation = _ACT_CODE[activation]
+    return args, lead
+
+
 def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, scales=None):
     """bf16 rows -> ``(codes, scales)``: int8 codes ``round(127 v / max|v|)`` (ties to even, correctly rounded) and fp32
     ``scales = max|v| / 127``, one per row ``v``; ``codes * scales`` is the row again.
@@ -653,43 +683,45 @@ def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, sc
     or a NaN has codes 0 and scale NaN, so every product of it is NaN.  Weights (G, N, K) give codes of that shape and
     scales (G, N).  ``codes`` / ``scales``: written in place when given.
     """
-    _require(x.is_cuda and x.dtype == torch.bfloat16, "quantize_rows_int8: x must be a CUDA bfloat16 tensor")
-    _require(x.dim() >= 2, "quantize_rows_int8: x must have at least two dimensions")
-    _no_grad_wanted("quantize_rows_int8", x)
-    if x.dim() > 2:
-        _require(x.is_contiguous() and indices is None, "quantize_rows_int8: x with more than two dimensions must be contiguous, without indices")
-    else:
-        _require(x.shape[1] <= 1 or x.stride(1) == 1, "quantize_rows_int8: the elements of a row must be contiguous")
-        _require(x.shape[0] <= 1 or x.stride(0) >= x.shape[1], "quantize_rows_int8: the rows of x overlap")
-    _require(activation in (None, "none", "gelu", "swiglu"), f"quantize_rows_int8: unknown activation {activation!r}")
-    width = x.shape[-1]
-    _require(activation != "swiglu" or width % 2 == 0, "quantize_rows_int8: swiglu needs [gate | up] columns")
-    cols = width // 2 if activation == "swiglu" else width
-    if indices is not None:
-        _require(indices.is_cuda and indices.device == x.device and indices.dtype == torch.int32 and indices.dim() == 1
-                 and indices.is_contiguous(), "quantize_rows_int8: indices must be a contiguous 1-D CUDA int32 tensor on the device of x")
-        _require(top_k >= 1, "quantize_rows_int8: top_k must be positive")
-        lead = (indices.numel(),)
-    else:
-        lead = tuple(x.shape[:-1])
+    args, lead = _quantize_args(x, indices, top_k, activation)
     if codes is None:
-        codes = torch.empty(*lead, cols, dtype=torch.int8, device=x.device)
+        codes = torch.empty(*lead, args.cols, dtype=torch.int8, device=x.device)
     if scales is None:
         scales = torch.empty(lead, dtype=torch.float32, device=x.device)
-    _require(codes.device == x.device and codes.dtype == torch.int8 and tuple(codes.shape) == lead + (cols,) and codes.is_contiguous(),
+    _require(codes.device == x.device and codes.dtype == torch.int8 and tuple(codes.shape) == lead + (args.cols,) and codes.is_contiguous(),
              "quantize_rows_int8: bad codes output")
     _require(scales.device == x.device and scales.dtype == torch.float32 and tuple(scales.shape) == lead and scales.is_contiguous(),
              "quantize_rows_int8: bad scales output")
-    args = QuantizeRowsArgs()
-    args.in_, args.in_ld = x.data_ptr(), x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else width
-    args.in_rows = math.prod(x.shape[:-1])
-    args.indices, args.top_k = _ptr(indices), int(top_k)
-    args.rows, args.cols = math.prod(lead), cols
-    args.activation = _ACT_CODE[activation]
     args.codes, args.scales = codes.data_ptr(), scales.data_ptr()
     with _on(x.device):
         check(lib.fp8gmm_quantize_rows_int8(ctypes.byref(args), _stream()), "quantize_rows_int8")
     return codes, scales
+
+
+def _int8_gemm_args(device, rows, k, b, group_sizes, b_scales, c, name):
+    """Checked arguments of the int8 product without a and its scales; the output; host memory to keep until the call."""
+    _require(b.device == device and b.dtype == torch.int8 and b.dim() == 3 and b.is_contiguous(),
+             f"{name}: the weights must be a contiguous 3-D int8 tensor on the device of the rows")
+    G, n, kb = b.shape
+    _require(kb == k, f"{name}: contraction dimensions differ")
+    _require(b_scales.device == device and b_scales.dtype == torch.float32 and b_scales.shape == (G, n) and b_scales.is_contiguous(),
+             f"{name}: the weights' scales must be (G, N) float32 on the device of the rows")
+    _require(len(group_sizes) == G, f"{name}: one group size per expert is required")
+    _no_grad_wanted(name, b_scales)
+    if c is None:
+        c = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+    _require(c.device == device and c.dtype == torch.bfloat16 and c.shape == (rows, n) and c.is_contiguous(), f"{name}: bad output")
+    args = Int8GemmArgs()
+    keep = None
+    if torch.is_tensor(group_sizes) and group_sizes.is_cuda:
+        _require(group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.dim() == 1 and group_sizes.is_contiguous(),
+                 f"{name}: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of the rows")
+        args.device_m_sizes = group_sizes.data_ptr()
+    else:
+        args.m_sizes, keep = _i64_array(group_sizes)
+    args.b, args.c, args.b_scales = b.data_ptr(), c.data_ptr(), b_scales.data_ptr()
+    args.num_groups, args.rows, args.n, args.k = G, rows, n, k
+    return args, c, keep
 
 
 def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
@@ -701,31 +733,12 @@ def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
     be captured into a graph and replayed with other sizes, and rows behind the last group are left as they are.
     """
     _require(a.is_cuda and a.dtype == torch.int8 and a.dim() == 2 and a.is_contiguous(), "int8_gmm: a must be a contiguous 2-D CUDA int8 tensor")
-    _require(b.device == a.device and b.dtype == torch.int8 and b.dim() == 3 and b.is_contiguous(),
-             "int8_gmm: b must be a contiguous 3-D int8 tensor on the device of a")
     rows, k = a.shape
-    G, n = b.shape[0], b.shape[1]
-    _require(b.shape[2] == k, "int8_gmm: contraction dimensions differ")
-    _require(a_scales.device == a.device and a_scales.dtype == torch.float32 and tuple(a_scales.shape) == (rows,) and a_scales.is_contiguous(),
+    _require(a_scales.device == a.device and a_scales.dtype == torch.float32 and a_scales.shape == (rows,) and a_scales.is_contiguous(),
              "int8_gmm: a_scales must be (rows,) float32 on the device of a")
-    _require(b_scales.device == a.device and b_scales.dtype == torch.float32 and tuple(b_scales.shape) == (G, n) and b_scales.is_contiguous(),
-             "int8_gmm: b_scales must be (G, N) float32 on the device of a")
-    _require(len(group_sizes) == G, "int8_gmm: one group size per expert is required")
-    _no_grad_wanted("int8_gmm", a_scales, b_scales)
-    if c is None:
-        c = torch.empty(rows, n, dtype=torch.bfloat16, device=a.device)
-    _require(c.device == a.device and c.dtype == torch.bfloat16 and tuple(c.shape) == (rows, n) and c.is_contiguous(), "int8_gmm: bad output")
-    args = Int8GemmArgs()
-    keep = None
-    if torch.is_tensor(group_sizes) and group_sizes.is_cuda:
-        _require(group_sizes.device == a.device and group_sizes.dtype == torch.int64 and group_sizes.dim() == 1 and group_sizes.is_contiguous(),
-                 "int8_gmm: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of a")
-        args.device_m_sizes = group_sizes.data_ptr()
-    else:
-        args.m_sizes, keep = _i64_array(group_sizes)
-    args.a, args.b, args.c = a.data_ptr(), b.data_ptr(), c.data_ptr()
-    args.a_scales, args.b_scales = a_scales.data_ptr(), b_scales.data_ptr()
-    args.num_groups, args.rows, args.n, args.k = G, rows, n, k
+    _no_grad_wanted("int8_gmm", a_scales)
+    args, c, keep = _int8_gemm_args(a.device, rows, k, b, group_sizes, b_scales, c, "int8_gmm")
+    args.a, args.a_scales = a.data_ptr(), a_scales.data_ptr()
     with _on(a.device):
         check(lib.fp8gmm_int8_grouped_gemm(ctypes.byref(args), _stream()), "int8_gmm")
     del keep
@@ -733,14 +746,23 @@ def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
 
 
 def int8_linear(x, weight, group_sizes, weight_scales, indices=None, top_k=1, activation=None, c=None):
-    """bf16 rows through int8 experts: ``quantize_rows_int8`` (with its gather and activation) and ``int8_gmm``.
+    """bf16 rows through int8 experts: ``quantize_rows_int8`` (with its gather and activation) and ``int8_gmm`` in one call, the
+    product loading weights while the rows are still being quantised.
 
     x: (rows, K) bf16 sorted by expert, or with ``indices`` the tokens (tokens, K) as the router sees them; weight
     (G, N, K) int8 with weight_scales (G, N) from ``quantize_rows_int8(weight)``.  Returns (rows, N) bf16, rows sorted by
     expert."""
     _require(x.dim() == 2, "int8_linear: x must be a matrix")
-    codes, scales = quantize_rows_int8(x, indices, top_k, activation)
-    return int8_gmm(codes, weight, group_sizes, scales, weight_scales, c)
+    q, (rows,) = _quantize_args(x, indices, top_k, activation)
+    k = q.cols
+    g, c, keep = _int8_gemm_args(x.device, rows, k, weight, group_sizes, weight_scales, c, "int8_linear")
+    scratch = torch.empty(rows * (k + 4), dtype=torch.int8, device=x.device)   # codes, then scales (K is a multiple of 16)
+    q.codes = g.a = scratch.data_ptr()
+    q.scales = g.a_scales = scratch.data_ptr() + rows * k
+    with _on(x.device):
+        check(lib.fp8gmm_int8_linear(ctypes.byref(q), ctypes.byref(g), _stream()), "int8_linear")
+    del keep
+    return c
 
 
 # ------------------------------------------------------------------------------------------------

@@ -19,6 +19,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "int8.cuh"
 #include "sm100_ptx.cuh"
 
 namespace fp8gmm {
@@ -44,8 +45,6 @@ struct Int8GemmParams {
   int tile_rows, tiles_n, super_tiles;
   int row_start[kMaxGroups + 1];
 };
-
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // D[tmem] (+)= W[smem] X[smem]^T in 8-bit integers, issued by one thread.
 template <int kCtas>
@@ -591,14 +590,19 @@ int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, 
 int g_tile_rows = 0, g_splits = 0;
 
 template <typename... Args>
-int launch(void (*kernel)(Args...), int grid, int cluster, int smem, cudaStream_t s, Args... args) {
+int launch(void (*kernel)(Args...), int grid, int cluster, int smem, cudaStream_t s, bool early, Args... args) {
   FP8GMM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  if (early) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
   if (cluster > 1) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
     attr[cfg.numAttrs].val.clusterDim.x = cluster;
@@ -612,29 +616,15 @@ int launch(void (*kernel)(Args...), int grid, int cluster, int smem, cudaStream_
 }
 
 template <int kT>
-int launch_stream(Int8GemmParams& p, int64_t row_tiles, int splits, cudaStream_t s) {
+int launch_stream(Int8GemmParams& p, int64_t row_tiles, int splits, cudaStream_t s, bool early) {
   const int64_t grid = row_tiles * p.tiles_n * splits;
   FP8GMM_CHECK_ARG(grid <= INT32_MAX, "int8_grouped_gemm: problem too large");
-  return launch<Int8GemmParams, int>(int8_stream_kernel<kT>, static_cast<int>(grid), splits, StreamCfg<kT>::kSmemBytes, s, p, splits);
+  return launch<Int8GemmParams, int>(int8_stream_kernel<kT>, static_cast<int>(grid), splits, StreamCfg<kT>::kSmemBytes, s, early, p, splits);
 }
 
 }  // namespace
-}  // namespace fp8gmm
-
-extern "C" {
-
-int fp8gmm_set_int8_variant(int tile_rows, int splits) {
-  using namespace fp8gmm;
-  FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 16 || tile_rows == 32 || tile_rows == 64 || tile_rows == 128 || tile_rows == 256,
-                   "set_int8_variant: tile_rows must be 0, 16, 32, 64, 128 or 256");
-  FP8GMM_CHECK_ARG(splits == 0 || splits == 1 || splits == 2 || splits == 4 || splits == 8, "set_int8_variant: splits must be 0, 1, 2, 4 or 8");
-  g_tile_rows = tile_rows;
-  g_splits = splits;
-  return FP8GMM_OK;
-}
-
-int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) {
-  using namespace fp8gmm;
+// Argument checks; nothing is launched and no CUDA call made.
+int int8_gemm_check(const fp8gmm_int8_gemm_args* a) {
   FP8GMM_CHECK_ARG(a != nullptr, "int8_grouped_gemm: NULL arguments");
   FP8GMM_CHECK_ARG(a->num_groups >= 0 && a->num_groups <= kMaxGroups, "int8_grouped_gemm: num_groups %d outside [0, %d]", a->num_groups, kMaxGroups);
   FP8GMM_CHECK_ARG(a->n > 0 && a->k > 0 && a->n % 16 == 0 && a->k % 16 == 0, "int8_grouped_gemm: N (%lld) and K (%lld) must be positive multiples of 16",
@@ -644,19 +634,27 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) {
   FP8GMM_CHECK_ARG(a->rows >= 0 && a->rows <= INT32_MAX - 1024, "int8_grouped_gemm: bad number of rows");
   FP8GMM_CHECK_ARG(a->num_groups == 0 || (a->m_sizes != nullptr) != (a->device_m_sizes != nullptr),
                    "int8_grouped_gemm: group sizes are given on the host or on the device, not both");
-  Int8GemmParams p;
-  memset(&p, 0, sizeof(p));
-  for (int g = 0; g < a->num_groups; ++g) {
-    const int64_t m = a->m_sizes != nullptr ? a->m_sizes[g] : 0;
-    FP8GMM_CHECK_ARG(m >= 0 && m <= a->rows - p.row_start[g], "int8_grouped_gemm: group %d has a bad size of %lld", g, (long long)m);
-    p.row_start[g + 1] = p.row_start[g] + static_cast<int>(m);
+  int64_t sum = 0;
+  for (int g = 0; a->m_sizes != nullptr && g < a->num_groups; ++g) {
+    const int64_t m = a->m_sizes[g];
+    FP8GMM_CHECK_ARG(m >= 0 && m <= a->rows - sum, "int8_grouped_gemm: group %d has a bad size of %lld", g, (long long)m);
+    sum += m;
   }
-  FP8GMM_CHECK_ARG(a->m_sizes == nullptr || p.row_start[a->num_groups] == a->rows, "int8_grouped_gemm: the group sizes sum to %d, not to the %lld rows",
-                   p.row_start[a->num_groups], (long long)a->rows);
+  FP8GMM_CHECK_ARG(a->m_sizes == nullptr || sum == a->rows, "int8_grouped_gemm: the group sizes sum to %lld, not to the %lld rows",
+                   (long long)sum, (long long)a->rows);
   if (a->rows == 0 || a->num_groups == 0) return FP8GMM_OK;
   FP8GMM_CHECK_ARG(a->a && a->b && a->c && a->a_scales && a->b_scales, "int8_grouped_gemm: NULL pointer");
   FP8GMM_CHECK_ARG((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->b) | reinterpret_cast<uintptr_t>(a->c)) % 16 == 0,
                    "int8_grouped_gemm: operand pointers must be 16-byte aligned");
+  return FP8GMM_OK;
+}
+
+int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_quantize) {
+  int rc = int8_gemm_check(a);
+  if (rc != FP8GMM_OK || a->rows == 0 || a->num_groups == 0) return rc;
+  Int8GemmParams p;
+  memset(&p, 0, sizeof(p));
+  for (int g = 0; a->m_sizes != nullptr && g < a->num_groups; ++g) p.row_start[g + 1] = p.row_start[g] + static_cast<int>(a->m_sizes[g]);
   p.c = static_cast<uint16_t*>(a->c);
   p.a_scales = a->a_scales;
   p.b_scales = a->b_scales;
@@ -674,7 +672,7 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) {
   int tile_rows = g_tile_rows;
   if (tile_rows == 0) tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
   p.tile_rows = tile_rows;
-  int rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, kChannels);
+  rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, kChannels);
   if (rc != FP8GMM_OK) return rc;
   rc = encode_rows(&p.map_x, a->a, a->rows, a->k, tile_rows == 256 ? 128 : tile_rows);
   if (rc != FP8GMM_OK) return rc;
@@ -688,7 +686,7 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) {
     p.super_tiles = (p.k > 8192 ? 2048 : 4096) / PairCfg::kRows;
     int sms = sm_count() / 2;
     const int64_t most = row_tiles * p.tiles_n;
-    return launch<Int8GemmParams>(int8_pair_kernel, 2 * static_cast<int>(most < sms ? most : sms), 1, PairCfg::kSmemBytes, s, p);
+    return launch<Int8GemmParams>(int8_pair_kernel, 2 * static_cast<int>(most < sms ? most : sms), 1, PairCfg::kSmemBytes, s, after_quantize, p);
   }
   p.super_tiles = INT32_MAX / 2 / p.tiles_n;   // row tiles fastest: the CTAs that share weights run side by side
   int splits = g_splits;
@@ -700,11 +698,36 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) {
   }
   while (splits > num_kb || splits > tile_rows) splits /= 2;
   switch (tile_rows) {
-    case 16: return launch_stream<16>(p, row_tiles, splits, s);
-    case 32: return launch_stream<32>(p, row_tiles, splits, s);
-    case 64: return launch_stream<64>(p, row_tiles, splits, s);
-    default: return launch_stream<128>(p, row_tiles, splits, s);
+    case 16: return launch_stream<16>(p, row_tiles, splits, s, after_quantize);
+    case 32: return launch_stream<32>(p, row_tiles, splits, s, after_quantize);
+    case 64: return launch_stream<64>(p, row_tiles, splits, s, after_quantize);
+    default: return launch_stream<128>(p, row_tiles, splits, s, after_quantize);
   }
+}
+}  // namespace fp8gmm
+
+extern "C" {
+
+int fp8gmm_set_int8_variant(int tile_rows, int splits) {
+  using namespace fp8gmm;
+  FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 16 || tile_rows == 32 || tile_rows == 64 || tile_rows == 128 || tile_rows == 256,
+                   "set_int8_variant: tile_rows must be 0, 16, 32, 64, 128 or 256");
+  FP8GMM_CHECK_ARG(splits == 0 || splits == 1 || splits == 2 || splits == 4 || splits == 8, "set_int8_variant: splits must be 0, 1, 2, 4 or 8");
+  g_tile_rows = tile_rows;
+  g_splits = splits;
+  return FP8GMM_OK;
+}
+
+int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) { return fp8gmm::int8_gemm_launch(a, stream, false); }
+
+int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gemm_args* g, void* stream) {
+  FP8GMM_CHECK_ARG(q != nullptr && g != nullptr, "int8_linear: NULL arguments");
+  FP8GMM_CHECK_ARG(q->codes == g->a && q->scales == g->a_scales && q->rows == g->rows && q->cols == g->k,
+                   "int8_linear: the product has to take the codes, scales, rows and columns of the quantisation");
+  int rc = fp8gmm::int8_gemm_check(g);   // before anything is launched
+  if (rc != FP8GMM_OK) return rc;
+  rc = fp8gmm_quantize_rows_int8(q, stream);
+  return rc != FP8GMM_OK ? rc : fp8gmm::int8_gemm_launch(g, stream, q->rows > 0);
 }
 
 }  // extern "C"

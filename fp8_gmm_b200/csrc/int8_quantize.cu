@@ -11,12 +11,18 @@
 // neither the reciprocal nor the product leaves fp32's range.
 // A row of zeros has scale 0 and codes 0.  A row that holds an infinity or a NaN has scale NaN and codes 0: all its products
 // come out NaN, no other row's do.
-#include "common.cuh"
+//
+// Two kernels.  quantize_rows_kernel: one CTA per row, the row in registers between the maximum and the codes, so it is read
+// once; 16-byte loads, 8-byte stores.  quantize_long_rows_kernel: rows that are too long for that, or not aligned to 16 bytes,
+// are walked twice (the second time out of L2 or L1).
+#include "int8.cuh"
 
 namespace fp8gmm {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kLongThreads = 256;
+constexpr int kMaxThreads = 512;
+constexpr int kMaxVecs = 4;              // 8-element vectors a thread holds: rows of up to 512 * 4 * 8 = 16384 elements
 constexpr int kStatusBadIndex = 0x200;   // as in routing.cu: an index that names no row
 
 struct QuantRowsParams {
@@ -33,11 +39,13 @@ struct QuantRowsParams {
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
 
+// The activation in fp32: hardware exp2 and division (a few ulp; their argument's rounding, |a| 2^-24, is larger from |a| = 4 on).
+// An exp that overflows gives a / inf = 0.
 template <int kAct>
 __device__ __forceinline__ float activated(float a, float b) {
-  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return a / (1.f + expf(-a)) * b;
+  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return __fdividef(a, 1.f + __expf(-a)) * b;
   // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)): without the cancellation of 1 + tanh u at negative u
-  if constexpr (kAct == FP8GMM_ACT_GELU) return a / (1.f + expf(-2.f * 0.79788456f * a * (1.f + 0.044715f * a * a)));
+  if constexpr (kAct == FP8GMM_ACT_GELU) return __fdividef(a, 1.f + __expf(-2.f * 0.79788456f * a * (1.f + 0.044715f * a * a)));
   return a;
 }
 
@@ -63,56 +71,128 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
   }
   return s;
 }
-__device__ __forceinline__ int code_of(float v, const RowScale& s) {
+// The code in the low byte: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.
+__device__ __forceinline__ uint32_t code_of(float v, const RowScale& s) {
   const float t = v * s.pre;
   float y = t * s.inv;
   y = fmaf(fmaf(-y, s.top, t), s.inv, y);
-  return __float2int_rn(y);
+  return __float_as_uint(y + 12582912.f);
 }
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {
-  __shared__ uint32_t warp_max_[kThreads / 32];
+// Maximum over the block; `warp_max` has a place for every warp.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* warp_max) {
   v = __reduce_max_sync(0xFFFFFFFFu, v);
-  if ((threadIdx.x & 31) == 0) warp_max_[threadIdx.x >> 5] = v;
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = v;
   __syncthreads();
-  uint32_t m = 0;
+  const int lane = threadIdx.x & 31;
+  return __reduce_max_sync(0xFFFFFFFFu, lane < warps ? warp_max[lane] : 0u);
+}
+
+// Source row of row r, or -1 (reported) if the index names none.
+__device__ __forceinline__ int64_t source_row(const QuantRowsParams& p, int64_t r) {
+  if (p.indices == nullptr) return r;
+  const int32_t slot = p.indices[r];
+  const int64_t src = slot / p.top_k;
+  if (slot >= 0 && src < p.in_rows) return src;
+  if (threadIdx.x == 0) atomicOr(p.status, kStatusBadIndex);
+  return -1;
+}
+
+template <int kAct, int kVecs>
+__global__ void __launch_bounds__(kMaxThreads) quantize_rows_kernel(const QuantRowsParams p) {
+  __shared__ uint32_t warp_max[kMaxThreads / 32];
+  let_dependents_start();
+  const int64_t r = blockIdx.x;
+  const int64_t src = source_row(p, r);
+  const int vecs = static_cast<int>(p.cols >> 3);
+  const uint4* a = reinterpret_cast<const uint4*>(p.in + (src < 0 ? 0 : src) * p.in_ld);
+  uint4 raw[kVecs], raw2[kAct == FP8GMM_ACT_SWIGLU ? kVecs : 1];
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) m = max(m, warp_max_[w]);
-  __syncthreads();
-  return m;
+  for (int u = 0; u < kVecs; ++u) {
+    const int c = threadIdx.x + u * blockDim.x;
+    const bool in = c < vecs && src >= 0;
+    raw[u] = in ? __ldg(a + c) : make_uint4(0, 0, 0, 0);
+    if constexpr (kAct == FP8GMM_ACT_SWIGLU) raw2[u] = in ? __ldg(a + vecs + c) : make_uint4(0, 0, 0, 0);   // [gate | up]
+  }
+  float v[kVecs][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+    uint32_t w2[4] = {0, 0, 0, 0};
+    if constexpr (kAct == FP8GMM_ACT_SWIGLU) w2[0] = raw2[u].x, w2[1] = raw2[u].y, w2[2] = raw2[u].z, w2[3] = raw2[u].w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[u][2 * j] = activated<kAct>(bf16_lo(w[j]), bf16_lo(w2[j]));
+      v[u][2 * j + 1] = activated<kAct>(bf16_hi(w[j]), bf16_hi(w2[j]));
+      // ordered as integers, with NaN above infinity
+      top = max(top, max(__float_as_uint(v[u][2 * j]) & 0x7FFFFFFFu, __float_as_uint(v[u][2 * j + 1]) & 0x7FFFFFFFu));
+    }
+  }
+  const RowScale s = row_scale(block_max(top, warp_max));
+  if (threadIdx.x == 0) p.scales[r] = s.scale;
+  const bool zero = s.pre == 0.f;
+  uint2* out = reinterpret_cast<uint2*>(p.codes + r * p.cols);
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int c = threadIdx.x + u * blockDim.x;
+    if (c >= vecs) break;
+    uint32_t q[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float* x = &v[u][4 * h];
+      const uint32_t lo = __byte_perm(code_of(x[0], s), code_of(x[1], s), 0x0040);
+      const uint32_t hi = __byte_perm(code_of(x[2], s), code_of(x[3], s), 0x0040);
+      q[h] = zero ? 0u : __byte_perm(lo, hi, 0x5410);
+    }
+    out[c] = make_uint2(q[0], q[1]);
+  }
 }
 
 template <int kAct>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantRowsParams p) {
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    int64_t src = r;
-    if (p.indices != nullptr) {
-      const int32_t slot = p.indices[r];
-      src = slot / p.top_k;
-      if (slot < 0 || src >= p.in_rows) {   // names no row: zeros, reported
-        if (threadIdx.x == 0) {
-          atomicOr(p.status, kStatusBadIndex);
-          p.scales[r] = 0.f;
-        }
-        for (int64_t c = threadIdx.x; c < p.cols; c += kThreads) p.codes[r * p.cols + c] = 0;
-        continue;
-      }
-    }
-    const uint16_t* a = p.in + src * p.in_ld;
+__global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const QuantRowsParams p) {
+  __shared__ uint32_t warp_max[2][kLongThreads / 32];
+  let_dependents_start();
+  int turn = 0;   // two sets of places: a warp may be one row ahead of another
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
+    const int64_t src = source_row(p, r);
+    const uint16_t* a = p.in + (src < 0 ? 0 : src) * p.in_ld;
     const uint16_t* b = a + p.cols;   // SwiGLU: [gate | up]
     uint32_t top = 0;
-    for (int64_t c = threadIdx.x; c < p.cols; c += kThreads) {
-      const float v = activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f);
-      top = max(top, __float_as_uint(v) & 0x7FFFFFFFu);   // ordered as integers, with NaN above infinity
-    }
-    const RowScale s = row_scale(block_max(top));
+    if (src >= 0)
+      for (int64_t c = threadIdx.x; c < p.cols; c += kLongThreads) {
+        const float v = activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f);
+        top = max(top, __float_as_uint(v) & 0x7FFFFFFFu);
+      }
+    const RowScale s = row_scale(block_max(top, warp_max[turn]));
     if (threadIdx.x == 0) p.scales[r] = s.scale;
     const bool zero = s.pre == 0.f;
-    for (int64_t c = threadIdx.x; c < p.cols; c += kThreads) {
-      const float v = activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f);
-      p.codes[r * p.cols + c] = static_cast<int8_t>(zero ? 0 : code_of(v, s));
+    for (int64_t c = threadIdx.x; c < p.cols; c += kLongThreads) {
+      uint32_t q = 0;
+      if (!zero) q = code_of(activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f), s);
+      p.codes[r * p.cols + c] = static_cast<int8_t>(q & 0xFFu);
     }
   }
+}
+
+template <int kAct>
+void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
+  const int64_t vecs = p.cols / 8;
+  const bool aligned = p.cols % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
+  if (aligned && vecs <= kMaxThreads * kMaxVecs && p.rows <= INT32_MAX) {
+    // as few vectors per thread as 512 threads allow: a row waits for its slowest load once
+    const int per = vecs <= kMaxThreads ? 1 : vecs <= 2 * kMaxThreads ? 2 : 4;
+    const int threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
+    const int grid = static_cast<int>(p.rows);
+    if (per == 1) quantize_rows_kernel<kAct, 1><<<grid, threads, 0, s>>>(p);
+    else if (per == 2) quantize_rows_kernel<kAct, 2><<<grid, threads, 0, s>>>(p);
+    else quantize_rows_kernel<kAct, 4><<<grid, threads, 0, s>>>(p);
+    return;
+  }
+  const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
+  quantize_long_rows_kernel<kAct><<<static_cast<int>(p.rows < cap ? p.rows : cap), kLongThreads, 0, s>>>(p);
 }
 
 }  // namespace
@@ -146,11 +226,9 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) 
   p.status = device_status_word();
   FP8GMM_CHECK_ARG(p.status != nullptr, "quantize_rows_int8: cannot resolve the device status word");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
-  const int grid = static_cast<int>(a->rows < cap ? a->rows : cap);
-  if (a->activation == FP8GMM_ACT_SWIGLU) quantize_rows_kernel<FP8GMM_ACT_SWIGLU><<<grid, kThreads, 0, s>>>(p);
-  else if (a->activation == FP8GMM_ACT_GELU) quantize_rows_kernel<FP8GMM_ACT_GELU><<<grid, kThreads, 0, s>>>(p);
-  else quantize_rows_kernel<FP8GMM_ACT_NONE><<<grid, kThreads, 0, s>>>(p);
+  if (a->activation == FP8GMM_ACT_SWIGLU) launch_rows<FP8GMM_ACT_SWIGLU>(p, s);
+  else if (a->activation == FP8GMM_ACT_GELU) launch_rows<FP8GMM_ACT_GELU>(p, s);
+  else launch_rows<FP8GMM_ACT_NONE>(p, s);
   FP8GMM_CHECK_CUDA(cudaGetLastError());
   count_launch();
   return FP8GMM_OK;

@@ -457,6 +457,10 @@ typedef struct {
 
 int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
 
+/* Both calls, the second on the codes and scales that the first writes (q->codes == g->a, q->scales == g->a_scales, the same
+ * rows and columns); the product starts loading weights while the rows are still being quantised. */
+int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gemm_args* g, void* stream);
+
 /* Process-wide switch of the launches above, for tests and experiments: rows of a tile (16, 32, 64, 128, or 256 = CTA pairs;
  * 0 = chosen per call, the default) and the CTAs that share the contraction of a tile of at most 128 rows (1, 2, 4, 8; 0 =
  * chosen per call).  Results are bit-identical. */
