@@ -35,7 +35,7 @@ COMMON = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
 ]
-HEADERS = ["common.cuh", "sm100_ptx.cuh", "int8.cuh", os.path.join("..", "..", "include", "fp8_gmm_b200.h")]
+HEADERS = ["common.cuh", "sm100_ptx.cuh", "int8.cuh", "dependent_launch.cuh", os.path.join("..", "..", "include", "fp8_gmm_b200.h")]
 
 
 def _nvcc():

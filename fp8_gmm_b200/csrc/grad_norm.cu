@@ -5,12 +5,17 @@
 // Two launches: every CTA of the first writes one partial sum of squares, in double, into a workspace slot of its own;
 // every CTA of the second adds up all slots in the same fixed order (so no atomics, and the same bits on every run) and
 // scales its share of the elements.  A tensor list travels in the kernel parameter block, as in pointwise.cu.
+// Squares: 8 elements are summed in fp32 and these sums added up in double.  An fp32 square overflows above 1.8e19 and loses
+// bits below 1e-19, both inside bf16's range; a thread whose fp32 sum of 32 elements is not in [2^-100, inf) therefore adds
+// them up again in double, out of registers (all zeros excepted, which empty experts leave).
+// The second launch walks the elements backwards: what the first one read last is still in L2, and its own results are stored
+// so that they leave L2 first.
 #include <algorithm>
 #include <cmath>
 #include <new>
 #include <vector>
 
-#include "common.cuh"
+#include "dependent_launch.cuh"
 
 #include <cuda_fp16.h>
 
@@ -18,15 +23,20 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTileElems = 8192;
+constexpr int kUnit = 8;                               // elements that a thread handles side by side
+constexpr int kUnits = 4;                              // units in flight per thread
+constexpr int kTileElems = kThreads * kUnit * kUnits;  // 8192
 constexpr int kMaxTensors = 320;
+constexpr int kCtasPerSm = 4;
 constexpr int kMaxGrid = 1024;  // workspace slots of one launch
 
 struct GradDesc {
   const void* in;
   void* out;
   int64_t numel;
-  int in_type, out_type;
+  int8_t in_type, out_type;
+  int8_t shift;    // elements by which `in` lies behind a 16-byte boundary: tiles start on the boundary
+  int8_t out_vec;  // `out` has 16-byte boundaries at the same elements
 };
 
 struct GradArgs {
@@ -35,15 +45,81 @@ struct GradArgs {
   GradDesc d[kMaxTensors];
 };
 
-__device__ __forceinline__ float load_elem(const void* p, int type, int64_t i) {
-  if (type == FP8GMM_F32) return static_cast<const float*>(p)[i];
-  if (type == FP8GMM_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void store_elem(void* p, int type, int64_t i, float v) {
-  if (type == FP8GMM_F32) static_cast<float*>(p)[i] = v;
-  else if (type == FP8GMM_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+// The raw bits of a thread's units of a tile; elements outside the tensor are 0.  Unit u holds elements
+// first + u * kThreads * kUnit + [0, kUnit).  All loads are issued before the first use.
+template <int kType>
+struct Units {
+  static constexpr int kWords = kType == FP8GMM_F32 ? 8 : 4;
+  uint32_t w[kUnits][kWords];
+
+  __device__ __forceinline__ void load(const GradDesc& d, int64_t first) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int64_t i = first + u * (kThreads * kUnit);
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const char*>(d.in) + i * (kType == FP8GMM_F32 ? 4 : 2));
+      if (i >= 0 && i + kUnit <= d.numel) {
+#pragma unroll
+        for (int h = 0; h < kWords; h += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p + h);
+          w[u][h] = x.x, w[u][h + 1] = x.y, w[u][h + 2] = x.z, w[u][h + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < kWords; ++h) w[u][h] = 0u;
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j)
+          if (i + j >= 0 && i + j < d.numel) {
+            if constexpr (kType == FP8GMM_F32) w[u][j] = p[j];
+            else w[u][j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[j]) << (16 * (j & 1));
+          }
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(int u, float (&v)[kUnit]) const {
+#pragma unroll
+    for (int h = 0; h < kWords; ++h) {
+      if constexpr (kType == FP8GMM_F32) {
+        v[h] = __uint_as_float(w[u][h]);
+      } else if constexpr (kType == FP8GMM_BF16) {
+        v[2 * h] = bf16_lo(w[u][h]);
+        v[2 * h + 1] = bf16_hi(w[u][h]);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[u][h]));
+        v[2 * h] = f.x;
+        v[2 * h + 1] = f.y;
+      }
+    }
+  }
+};
+
+// Stores elements i + [0, kUnit), those that lie in the tensor.
+template <int kType>
+__device__ __forceinline__ void store_unit(const GradDesc& d, int64_t i, const float (&v)[kUnit]) {
+  constexpr int kWords = kType == FP8GMM_F32 ? 8 : 4;
+  uint32_t w[kWords];
+#pragma unroll
+  for (int h = 0; h < kWords; ++h) {
+    if constexpr (kType == FP8GMM_F32) {
+      w[h] = __float_as_uint(v[h]);
+    } else if constexpr (kType == FP8GMM_BF16) {
+      w[h] = pack_bf16x2(v[2 * h], v[2 * h + 1]);
+    } else {
+      const __half2 x = __floats2half2_rn(v[2 * h], v[2 * h + 1]);
+      w[h] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+  }
+  uint32_t* p = reinterpret_cast<uint32_t*>(static_cast<char*>(d.out) + i * (kType == FP8GMM_F32 ? 4 : 2));
+  if (d.out_vec && i >= 0 && i + kUnit <= d.numel) {
+#pragma unroll
+    for (int h = 0; h < kWords; h += 4) st_stream16(p + h, make_uint4(w[h], w[h + 1], w[h + 2], w[h + 3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j)
+      if (i + j >= 0 && i + j < d.numel) {
+        if constexpr (kType == FP8GMM_F32) p[j] = w[j];
+        else reinterpret_cast<uint16_t*>(p)[j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+      }
+  }
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -55,23 +131,58 @@ __device__ __forceinline__ double block_sum(double v) {
   double total = 0.0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += warp_sums[w];
-  __syncthreads();
   return total;
 }
 
-// Squares in double: an fp32 square overflows above 1.8e19 and vanishes below 1e-23, both inside bf16's range.
-__global__ void __launch_bounds__(kThreads) sum_squares_kernel(const __grid_constant__ GradArgs args, double* __restrict__ partials) {
+__device__ __forceinline__ int64_t first_of(const GradArgs& args, int t, int tile) {
+  return static_cast<int64_t>(tile - args.tile_start[t]) * kTileElems - args.d[t].shift + threadIdx.x * kUnit;
+}
+
+template <int kType>
+__device__ __forceinline__ double tile_squares(const GradDesc& d, int64_t first) {
+  Units<kType> x;
+  x.load(d, first);
+  float s[kUnits], v[kUnit];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    x.unpack(u, v);
+    s[u] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) s[u] = fmaf(v[j], v[j], s[u]);
+  }
+  const float all = (s[0] + s[1]) + (s[2] + s[3]);
+  static_assert(kUnits == 4, "four partial sums");
+  // 2^-100 <= all < inf: no square overflowed, and what vanished is below 2^-45 of it
+  if (all >= 7.9e-31f && all <= 3.4e38f) return (static_cast<double>(s[0]) + s[1]) + (static_cast<double>(s[2]) + s[3]);
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+    for (int h = 0; h < Units<kType>::kWords; ++h) any |= x.w[u][h];
+  double sum = 0.0;
+  if (any != 0u) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      x.unpack(u, v);
+#pragma unroll
+      for (int j = 0; j < kUnit; ++j) sum = fma(static_cast<double>(v[j]), static_cast<double>(v[j]), sum);
+    }
+  }
+  return sum;
+}
+
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) sum_squares_kernel(const __grid_constant__ GradArgs args, double* __restrict__ partials) {
+  let_dependents_start();
   double sum = 0.0;
   const int tiles = args.tile_start[args.num];
+  int t = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int t = upper_slot(args.tile_start, args.num, tile);
+    while (args.tile_start[t + 1] <= tile) ++t;
     const GradDesc& d = args.d[t];
-    const int64_t base = static_cast<int64_t>(tile - args.tile_start[t]) * kTileElems;
-    const int64_t end = min(base + kTileElems, d.numel);
-    for (int64_t i = base + threadIdx.x; i < end; i += kThreads) {
-      const double v = load_elem(d.in, d.in_type, i);
-      sum += v * v;
-    }
+    const int64_t first = first_of(args, t, tile);
+    if (d.in_type == FP8GMM_BF16) sum += tile_squares<FP8GMM_BF16>(d, first);
+    else if (d.in_type == FP8GMM_F32) sum += tile_squares<FP8GMM_F32>(d, first);
+    else sum += tile_squares<FP8GMM_F16>(d, first);
   }
   sum = block_sum(sum);
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
@@ -85,6 +196,7 @@ __device__ __forceinline__ double total_of(const double* __restrict__ sums, int 
 
 __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partials, int num_partials,
                                                         double* __restrict__ sum, float* __restrict__ norm) {
+  grid_dependency_wait();
   const double total = total_of(partials, num_partials);
   if (threadIdx.x == 0) {
     if (sum != nullptr) *sum = total;
@@ -92,20 +204,41 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict
   }
 }
 
-__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ GradArgs args, const double* __restrict__ sums,
-                                                        int num_sums, float max_norm, float* __restrict__ norm) {
+template <int kType>
+__device__ __forceinline__ void clip_tile(const GradDesc& d, int64_t first, float coef) {
+  Units<kType> x;
+  x.load(d, first);
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t i = first + u * (kThreads * kUnit);
+    float v[kUnit];
+    x.unpack(u, v);
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) v[j] *= coef;
+    if (d.out_type == FP8GMM_BF16) store_unit<FP8GMM_BF16>(d, i, v);
+    else if (d.out_type == FP8GMM_F32) store_unit<FP8GMM_F32>(d, i, v);
+    else store_unit<FP8GMM_F16>(d, i, v);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_kernel(const __grid_constant__ GradArgs args, const double* __restrict__ sums,
+                                                                    int num_sums, float max_norm, float* __restrict__ norm) {
+  grid_dependency_wait();
   const double n = sqrt(total_of(sums, num_sums));
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
   const double c = static_cast<double>(max_norm) / (n + 1e-6);
   const float coef = c >= 1.0 ? 1.f : static_cast<float>(c);  // a NaN norm keeps its NaN
   const int tiles = args.tile_start[args.num];
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int t = upper_slot(args.tile_start, args.num, tile);
+  int t = args.num - 1;
+  for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+    const int tile = tiles - 1 - i;
+    while (args.tile_start[t] > tile) --t;
     const GradDesc& d = args.d[t];
-    const int64_t base = static_cast<int64_t>(tile - args.tile_start[t]) * kTileElems;
-    const int64_t end = min(base + kTileElems, d.numel);
-    for (int64_t i = base + threadIdx.x; i < end; i += kThreads)
-      store_elem(d.out, d.out_type, i, load_elem(d.in, d.in_type, i) * coef);
+    if (coef == 1.f && d.in == d.out) continue;   // in place and within the limit: nothing changes
+    const int64_t first = first_of(args, t, tile);
+    if (d.in_type == FP8GMM_BF16) clip_tile<FP8GMM_BF16>(d, first, coef);
+    else if (d.in_type == FP8GMM_F32) clip_tile<FP8GMM_F32>(d, first, coef);
+    else clip_tile<FP8GMM_F16>(d, first, coef);
   }
 }
 
@@ -168,9 +301,14 @@ int fill(GradArgs& args, const fp8gmm_grad_desc* descs, int i, int count) {
   for (; i < count && args.num < kMaxTensors; ++i) {
     const fp8gmm_grad_desc& t = descs[i];
     if (t.numel == 0) continue;
-    const int64_t tiles = (t.numel + kTileElems - 1) / kTileElems;
+    const int size = static_cast<int>(elem_size(t.in_type));
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(t.in) % 16) / size;
+    const int64_t tiles = (t.numel + shift + kTileElems - 1) / kTileElems;
     if (tiles + args.tile_start[args.num] > INT32_MAX) break;
-    args.d[args.num] = {t.in, t.out, t.numel, t.in_type, t.out_type};
+    GradDesc& d = args.d[args.num];
+    d = {t.in, t.out, t.numel, static_cast<int8_t>(t.in_type), static_cast<int8_t>(t.out_type), static_cast<int8_t>(shift), 0};
+    // as integers: `out` may be a NULL that is not used
+    if (type_ok(t.out_type)) d.out_vec = (reinterpret_cast<uintptr_t>(t.out) - static_cast<uintptr_t>(shift) * elem_size(t.out_type)) % 16 == 0;
     args.tile_start[args.num + 1] = args.tile_start[args.num] + static_cast<int>(tiles);
     ++args.num;
   }
@@ -178,7 +316,7 @@ int fill(GradArgs& args, const fp8gmm_grad_desc* descs, int i, int count) {
 }
 
 int grid_of(const GradArgs& args) {
-  const int cap = std::min(kMaxGrid, sm_count() * 4);
+  const int cap = std::min(kMaxGrid, sm_count() * kCtasPerSm);
   return std::min(args.tile_start[args.num], cap);
 }
 
@@ -199,19 +337,20 @@ int launch_sum_squares(const fp8gmm_grad_desc* descs, int count, double* partial
   return FP8GMM_OK;
 }
 
-int launch_clip(const fp8gmm_grad_desc* descs, int count, const double* sums, int num_sums, float max_norm, float* norm, cudaStream_t s) {
+int launch_clip(const fp8gmm_grad_desc* descs, int count, const double* sums, int num_sums, float max_norm, float* norm, bool after_sums, cudaStream_t s) {
   GradArgs args;
   for (int i = 0; i < count;) {
     i = fill(args, descs, i, count);
     if (args.num == 0) continue;
-    clip_kernel<<<grid_of(args), kThreads, 0, s>>>(args, sums, num_sums, max_norm, norm);
-    FP8GMM_CHECK_CUDA(cudaGetLastError());
+    // the first launch may follow the sums directly; a later one writes what the one before it may not have read yet only if
+    // an entry's output were another's input, which is refused
+    FP8GMM_CHECK_CUDA(launch_dependent(clip_kernel, grid_of(args), kThreads, 0, s, after_sums, args, sums, num_sums, max_norm, norm));
     count_launch();
+    after_sums = false;
     norm = nullptr;
   }
   if (norm != nullptr) {  // nothing to clip: the norm is still wanted
-    norm_kernel<<<1, kThreads, 0, s>>>(sums, num_sums, nullptr, norm);
-    FP8GMM_CHECK_CUDA(cudaGetLastError());
+    FP8GMM_CHECK_CUDA(launch_dependent(norm_kernel, 1, kThreads, 0, s, false, sums, num_sums, static_cast<double*>(nullptr), norm));
     count_launch();
   }
   return FP8GMM_OK;
@@ -246,8 +385,7 @@ int fp8gmm_multi_sum_squares(const fp8gmm_grad_desc* descs, int count, void* wor
   int used = 0;
   rc = launch_sum_squares(descs, count, static_cast<double*>(workspace), static_cast<int>(workspace_bytes / sizeof(double)), &used, s);
   if (rc != FP8GMM_OK) return rc;
-  norm_kernel<<<1, kThreads, 0, s>>>(static_cast<const double*>(workspace), used, sum, norm);
-  FP8GMM_CHECK_CUDA(cudaGetLastError());
+  FP8GMM_CHECK_CUDA(launch_dependent(norm_kernel, 1, kThreads, 0, s, used > 0, static_cast<const double*>(workspace), used, sum, norm));
   count_launch();
   return FP8GMM_OK;
 }
@@ -260,7 +398,7 @@ int fp8gmm_multi_clip(const fp8gmm_grad_desc* descs, int count, const double* su
   FP8GMM_CHECK_ARG(max_norm >= 0.f, "multi_clip: max_norm must not be negative");
   rc = check_overlap(descs, count, "multi_clip");
   if (rc != FP8GMM_OK) return rc;
-  return launch_clip(descs, count, sum, 1, max_norm, norm, static_cast<cudaStream_t>(stream));
+  return launch_clip(descs, count, sum, 1, max_norm, norm, false, static_cast<cudaStream_t>(stream));
 }
 
 int fp8gmm_multi_clip_grad_norm(const fp8gmm_grad_desc* descs, int count, float max_norm, void* workspace, size_t workspace_bytes,
@@ -277,7 +415,7 @@ int fp8gmm_multi_clip_grad_norm(const fp8gmm_grad_desc* descs, int count, float 
   int used = 0;
   rc = launch_sum_squares(descs, count, static_cast<double*>(workspace), static_cast<int>(workspace_bytes / sizeof(double)), &used, s);
   if (rc != FP8GMM_OK) return rc;
-  return launch_clip(descs, count, static_cast<const double*>(workspace), used, max_norm, norm, s);
+  return launch_clip(descs, count, static_cast<const double*>(workspace), used, max_norm, norm, used > 0, s);
 }
 
 }  // extern "C"
