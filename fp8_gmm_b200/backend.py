@@ -75,10 +75,10 @@ def set_gemm_variant(ctas=0, tail_split=True, tma_epilogue=True):
     check(lib.fp8gmm_set_gemm_variant(int(ctas), int(bool(tail_split)), int(bool(tma_epilogue))), "set_gemm_variant")
 
 
-def set_int8_variant(tile_rows=0, splits=0):
-    """Force the tile of the int8 product (rows of a tile: 16, 32, 64, 128 or 256; CTAs that share its contraction: 1, 2, 4 or
-    8; 0 = automatic); see fp8gmm_set_int8_variant.  For tests and experiments: results are bit-identical."""
-    check(lib.fp8gmm_set_int8_variant(int(tile_rows), int(splits)), "set_int8_variant")
+def set_int8_variant(tile_rows=0, split=True):
+    """Force the rows of the int8 product's tiles (64, 128 or 256; 0 = automatic), and forbid splitting the tiles of a
+    partial wave; see fp8gmm_set_int8_variant.  For tests and experiments: results are bit-identical."""
+    check(lib.fp8gmm_set_int8_variant(int(tile_rows), int(split)), "set_int8_variant")
 
 
 def set_wait_limits(gemm_wait_s=0.0, peer_wait_s=0.0):
@@ -631,46 +631,66 @@ def grouped_wgrad_rowmajor(dy, x, row_offsets, a_scale_invs, b_scale_invs, c=Non
 # products of 8-bit integers with scales per row and per output channel (evaluation and serving; no counterpart in the
 # reference, which has FP8 only)
 # ------------------------------------------------------------------------------------------------
+# The calls below can be as short as a few microseconds on the GPU, so their checks build no message unless they fail.
+_NOTHING = contextlib.nullcontext()
+
+
 def _on(device):
     """Context in which ``device`` is the current one: the launches below go to the stream of their tensors' device."""
     if _raw_device is not None and _raw_device() == device.index:
-        return contextlib.nullcontext()
+        return _NOTHING
     return torch.cuda.device(device)
 
 
-def _no_grad_wanted(name, *tensors):
-    _require(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)),
-             f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+def _fail(msg):
+    raise RuntimeError(msg)
+
+
+def _no_grad_wanted(name, tensor):
+    if tensor.requires_grad and torch.is_grad_enabled():
+        _fail(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _quantize_args(x, indices, top_k, activation):
     """Checked arguments of the row quantisation without its outputs, and the leading shape of those."""
-    _require(x.is_cuda and x.dtype == torch.bfloat16, "quantize_rows_int8: x must be a CUDA bfloat16 tensor")
-    dim, shape = x.dim(), x.shape
-    _require(dim >= 2, "quantize_rows_int8: x must have at least two dimensions")
+    if not (x.is_cuda and x.dtype == torch.bfloat16):
+        _fail("quantize_rows_int8: x must be a CUDA bfloat16 tensor")
+    shape = x.shape
+    dim = len(shape)
+    if dim < 2:
+        _fail("quantize_rows_int8: x must have at least two dimensions")
     _no_grad_wanted("quantize_rows_int8", x)
+    width = pitch = shape[-1]
     if dim > 2:
-        _require(x.is_contiguous() and indices is None, "quantize_rows_int8: x with more than two dimensions must be contiguous, without indices")
+        if not x.is_contiguous() or indices is not None:
+            _fail("quantize_rows_int8: x with more than two dimensions must be contiguous, without indices")
     else:
-        _require(shape[1] <= 1 or x.stride(1) == 1, "quantize_rows_int8: the elements of a row must be contiguous")
-        _require(shape[0] <= 1 or x.stride(0) >= shape[1], "quantize_rows_int8: the rows of x overlap")
-    _require(activation in (None, "none", "gelu", "swiglu"), f"quantize_rows_int8: unknown activation {activation!r}")
-    width = shape[-1]
-    _require(activation != "swiglu" or width % 2 == 0, "quantize_rows_int8: swiglu needs [gate | up] columns")
+        pitch, step = x.stride()
+        if step != 1 and width > 1:
+            _fail("quantize_rows_int8: the elements of a row must be contiguous")
+        if shape[0] <= 1:
+            pitch = width
+        elif pitch < width:
+            _fail("quantize_rows_int8: the rows of x overlap")
+    code = _ACT_CODE.get(activation)
+    if code is None:
+        _fail(f"quantize_rows_int8: unknown activation {activation!r}")
+    if code == ACT_SWIGLU and width % 2:
+        _fail("quantize_rows_int8: swiglu needs [gate | up] columns")
     args = QuantizeRowsArgs()
+    args.in_rows = args.rows = shape[0] if dim == 2 else math.prod(shape[:-1])
+    lead = shape[:-1]
     if indices is not None:
-        _require(indices.is_cuda and indices.device == x.device and indices.dtype == torch.int32 and indices.dim() == 1
-                 and indices.is_contiguous(), "quantize_rows_int8: indices must be a contiguous 1-D CUDA int32 tensor on the device of x")
-        _require(top_k >= 1, "quantize_rows_int8: top_k must be positive")
-        args.indices, args.top_k = indices.data_ptr(), int(top_k)
-        lead = tuple(indices.shape)
-    else:
-        lead = tuple(shape[:-1])
-    args.in_, args.in_ld = x.data_ptr(), x.stride(0) if dim == 2 and shape[0] > 1 else width
-    args.in_rows, args.rows = math.prod(shape[:-1]), math.prod(lead)
-    args.cols = width // 2 if activation == "swiglu" else width
-    args.activation = _ACT_CODE[activation]
-    return args, lead
+        if not (indices.dtype == torch.int32 and indices.device == x.device and indices.dim() == 1 and indices.is_contiguous()):
+            _fail("quantize_rows_int8: indices must be a contiguous 1-D CUDA int32 tensor on the device of x")
+        if top_k < 1:
+            _fail("quantize_rows_int8: top_k must be positive")
+        lead = indices.shape
+        args.indices, args.top_k, args.rows = indices.data_ptr(), int(top_k), lead[0]
+    args.in_, args.in_ld = x.data_ptr(), pitch
+    args.cols = width // 2 if code == ACT_SWIGLU else width
+    args.activation = code
+    return args, tuple(lead)
 
 
 def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, scales=None):
@@ -686,12 +706,12 @@ def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, sc
     args, lead = _quantize_args(x, indices, top_k, activation)
     if codes is None:
         codes = torch.empty(*lead, args.cols, dtype=torch.int8, device=x.device)
+    elif not (codes.device == x.device and codes.dtype == torch.int8 and tuple(codes.shape) == lead + (args.cols,) and codes.is_contiguous()):
+        _fail("quantize_rows_int8: bad codes output")
     if scales is None:
         scales = torch.empty(lead, dtype=torch.float32, device=x.device)
-    _require(codes.device == x.device and codes.dtype == torch.int8 and tuple(codes.shape) == lead + (args.cols,) and codes.is_contiguous(),
-             "quantize_rows_int8: bad codes output")
-    _require(scales.device == x.device and scales.dtype == torch.float32 and tuple(scales.shape) == lead and scales.is_contiguous(),
-             "quantize_rows_int8: bad scales output")
+    elif not (scales.device == x.device and scales.dtype == torch.float32 and tuple(scales.shape) == lead and scales.is_contiguous()):
+        _fail("quantize_rows_int8: bad scales output")
     args.codes, args.scales = codes.data_ptr(), scales.data_ptr()
     with _on(x.device):
         check(lib.fp8gmm_quantize_rows_int8(ctypes.byref(args), _stream()), "quantize_rows_int8")
@@ -700,22 +720,25 @@ def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, sc
 
 def _int8_gemm_args(device, rows, k, b, group_sizes, b_scales, c, name):
     """Checked arguments of the int8 product without a and its scales; the output; host memory to keep until the call."""
-    _require(b.device == device and b.dtype == torch.int8 and b.dim() == 3 and b.is_contiguous(),
-             f"{name}: the weights must be a contiguous 3-D int8 tensor on the device of the rows")
+    if not (b.device == device and b.dtype == torch.int8 and b.dim() == 3 and b.is_contiguous()):
+        _fail(f"{name}: the weights must be a contiguous 3-D int8 tensor on the device of the rows")
     G, n, kb = b.shape
-    _require(kb == k, f"{name}: contraction dimensions differ")
-    _require(b_scales.device == device and b_scales.dtype == torch.float32 and b_scales.shape == (G, n) and b_scales.is_contiguous(),
-             f"{name}: the weights' scales must be (G, N) float32 on the device of the rows")
-    _require(len(group_sizes) == G, f"{name}: one group size per expert is required")
+    if kb != k:
+        _fail(f"{name}: contraction dimensions differ")
+    if not (b_scales.device == device and b_scales.dtype == torch.float32 and b_scales.shape == (G, n) and b_scales.is_contiguous()):
+        _fail(f"{name}: the weights' scales must be (G, N) float32 on the device of the rows")
+    if len(group_sizes) != G:
+        _fail(f"{name}: one group size per expert is required")
     _no_grad_wanted(name, b_scales)
     if c is None:
         c = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
-    _require(c.device == device and c.dtype == torch.bfloat16 and c.shape == (rows, n) and c.is_contiguous(), f"{name}: bad output")
+    elif not (c.device == device and c.dtype == torch.bfloat16 and c.shape == (rows, n) and c.is_contiguous()):
+        _fail(f"{name}: bad output")
     args = Int8GemmArgs()
     keep = None
     if torch.is_tensor(group_sizes) and group_sizes.is_cuda:
-        _require(group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.dim() == 1 and group_sizes.is_contiguous(),
-                 f"{name}: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of the rows")
+        if not (group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.dim() == 1 and group_sizes.is_contiguous()):
+            _fail(f"{name}: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of the rows")
         args.device_m_sizes = group_sizes.data_ptr()
     else:
         args.m_sizes, keep = _i64_array(group_sizes)
@@ -734,12 +757,16 @@ def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
     """
     _require(a.is_cuda and a.dtype == torch.int8 and a.dim() == 2 and a.is_contiguous(), "int8_gmm: a must be a contiguous 2-D CUDA int8 tensor")
     rows, k = a.shape
-    _require(a_scales.device == a.device and a_scales.dtype == torch.float32 and a_scales.shape == (rows,) and a_scales.is_contiguous(),
-             "int8_gmm: a_scales must be (rows,) float32 on the device of a")
+    if not (a_scales.device == a.device and a_scales.dtype == torch.float32 and a_scales.shape == (rows,) and a_scales.is_contiguous()):
+        _fail("int8_gmm: a_scales must be (rows,) float32 on the device of a")
     _no_grad_wanted("int8_gmm", a_scales)
     args, c, keep = _int8_gemm_args(a.device, rows, k, b, group_sizes, b_scales, c, "int8_gmm")
     args.a, args.a_scales = a.data_ptr(), a_scales.data_ptr()
     with _on(a.device):
+        # taken per call, not kept: graphs captured one after the other would share a buffer that is kept
+        args.workspace_bytes = nbytes = lib.fp8gmm_int8_workspace_bytes(ctypes.byref(args))
+        ws = torch.empty(nbytes, dtype=torch.int8, device=a.device) if nbytes else None
+        args.workspace = _ptr(ws)
         check(lib.fp8gmm_int8_grouped_gemm(ctypes.byref(args), _stream()), "int8_gmm")
     del keep
     return c
@@ -756,10 +783,13 @@ def int8_linear(x, weight, group_sizes, weight_scales, indices=None, top_k=1, ac
     q, (rows,) = _quantize_args(x, indices, top_k, activation)
     k = q.cols
     g, c, keep = _int8_gemm_args(x.device, rows, k, weight, group_sizes, weight_scales, c, "int8_linear")
-    scratch = torch.empty(rows * (k + 4), dtype=torch.int8, device=x.device)   # codes, then scales (K is a multiple of 16)
-    q.codes = g.a = scratch.data_ptr()
-    q.scales = g.a_scales = scratch.data_ptr() + rows * k
     with _on(x.device):
+        # one buffer per call: the product's workspace, the codes, their scales (K is a multiple of 16)
+        g.workspace_bytes = nbytes = lib.fp8gmm_int8_workspace_bytes(ctypes.byref(g)) + 15 & -16
+        scratch = torch.empty(nbytes + rows * (k + 4), dtype=torch.int8, device=x.device)
+        g.workspace = scratch.data_ptr()
+        q.codes = g.a = g.workspace + nbytes if rows else None
+        q.scales = g.a_scales = g.a + rows * k if rows else None
         check(lib.fp8gmm_int8_linear(ctypes.byref(q), ctypes.byref(g), _stream()), "int8_linear")
     del keep
     return c
@@ -785,24 +815,31 @@ def _dense(t):
 
 def _grad_descs(grads, outputs, name):
     """Descriptor array (fp8gmm_grad_desc: in, out, numel, in_type | out_type << 32) and the common device."""
-    device = grads[0].device
+    index = grads[0].get_device() if grads[0].is_cuda else None
+    if outputs is not None and len(outputs) != len(grads):
+        _fail(f"{name}: one output per gradient is required")
     rows = []
-    _require(outputs is None or len(outputs) == len(grads), f"{name}: one output per gradient is required")
     for i, g in enumerate(grads):
         kind = _GRAD_TYPE.get(g.dtype)
-        _require(kind is not None and g.is_cuda and g.layout == torch.strided, f"{name}: gradient {i} must be a dense CUDA bfloat16, float16 or float32 tensor")
-        _require(g.device == device, f"{name}: gradient {i} is on another device than gradient 0")
-        _require(_dense(g), f"{name}: gradient {i} has gaps or shares elements with itself")
-        if outputs is None:
-            rows += (g.data_ptr(), g.data_ptr(), g.numel(), kind | kind << 32)
-        else:
+        if kind is None or not g.is_cuda or g.layout is not torch.strided:
+            _fail(f"{name}: gradient {i} must be a dense CUDA bfloat16, float16 or float32 tensor")
+        if g.get_device() != index:
+            _fail(f"{name}: gradient {i} is on another device than gradient 0")
+        plain = g.is_contiguous()
+        if not plain and not _dense(g):
+            _fail(f"{name}: gradient {i} has gaps or shares elements with itself")
+        ptr = out_ptr = g.data_ptr()
+        out_kind = kind
+        if outputs is not None:
             o = outputs[i]
             out_kind = _GRAD_TYPE.get(o.dtype)
-            _require(out_kind is not None and o.device == device, f"{name}: output {i} must be a bfloat16, float16 or float32 tensor on the device of the gradients")
-            _require(o.shape == g.shape and (o.is_contiguous() and g.is_contiguous() or o.stride() == g.stride()),
-                     f"{name}: output {i} does not have the layout of its gradient")
-            rows += (g.data_ptr(), o.data_ptr(), g.numel(), kind | out_kind << 32)
-    return np.array(rows, dtype=np.int64), device
+            if out_kind is None or not o.is_cuda or o.get_device() != index:
+                _fail(f"{name}: output {i} must be a bfloat16, float16 or float32 tensor on the device of the gradients")
+            if o.shape != g.shape or not (plain and o.is_contiguous() or o.stride() == g.stride()):
+                _fail(f"{name}: output {i} does not have the layout of its gradient")
+            out_ptr = o.data_ptr()
+        rows += (ptr, out_ptr, g.numel(), kind | out_kind << 32)
+    return (ctypes.c_int64 * len(rows))(*rows), grads[0].device
 
 
 def _grad_workspace(count, device):
@@ -820,7 +857,7 @@ def multi_sum_squares(grads):
     descs, device = _grad_descs(grads, None, "multi_sum_squares")
     with _on(device):
         ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_sum_squares(descs.ctypes.data, len(grads), ws.data_ptr(), ws.numel() * 8, out.data_ptr(), None, _stream()),
+        check(lib.fp8gmm_multi_sum_squares(descs, len(grads), ws.data_ptr(), ws.numel() * 8, out.data_ptr(), None, _stream()),
               "multi_sum_squares")
     return out
 
@@ -834,7 +871,7 @@ def multi_grad_norm(grads):
     descs, device = _grad_descs(grads, None, "multi_grad_norm")
     with _on(device):
         ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_sum_squares(descs.ctypes.data, len(grads), ws.data_ptr(), ws.numel() * 8, None, out.data_ptr(), _stream()),
+        check(lib.fp8gmm_multi_sum_squares(descs, len(grads), ws.data_ptr(), ws.numel() * 8, None, out.data_ptr(), _stream()),
               "multi_grad_norm")
     return out
 
@@ -853,10 +890,10 @@ def multi_clip(grads, sum_squares, max_norm, outputs=None):
     _require(sum_squares.is_cuda and sum_squares.dtype == torch.float64 and sum_squares.numel() == 1, "multi_clip: sum_squares must be one CUDA float64 value")
     max_norm = _max_norm(max_norm, "multi_clip")
     norm = torch.empty((), dtype=torch.float32, device=sum_squares.device)
-    descs, device = _grad_descs(grads, outputs, "multi_clip") if grads else (np.zeros(0, np.int64), sum_squares.device)
+    descs, device = _grad_descs(grads, outputs, "multi_clip") if grads else ((ctypes.c_int64 * 0)(), sum_squares.device)
     _require(device == sum_squares.device, "multi_clip: sum_squares is on another device than the gradients")
     with _on(device):
-        check(lib.fp8gmm_multi_clip(descs.ctypes.data, len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr(), _stream()), "multi_clip")
+        check(lib.fp8gmm_multi_clip(descs, len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr(), _stream()), "multi_clip")
     return norm
 
 
@@ -871,7 +908,7 @@ def multi_clip_grad_norm(grads, max_norm, outputs=None):
     descs, device = _grad_descs(grads, outputs, "multi_clip_grad_norm")
     with _on(device):
         ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_clip_grad_norm(descs.ctypes.data, len(grads), max_norm, ws.data_ptr(), ws.numel() * 8, norm.data_ptr(), _stream()),
+        check(lib.fp8gmm_multi_clip_grad_norm(descs, len(grads), max_norm, ws.data_ptr(), ws.numel() * 8, norm.data_ptr(), _stream()),
               "multi_clip_grad_norm")
     return norm
 

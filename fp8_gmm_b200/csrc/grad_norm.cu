@@ -27,6 +27,7 @@ constexpr int kUnit = 8;                               // elements that a thread
 constexpr int kUnits = 4;                              // units in flight per thread
 constexpr int kTileElems = kThreads * kUnit * kUnits;  // 8192
 constexpr int kMaxTensors = 320;
+constexpr int kFewTensors = 24;  // lists up to this length travel in a parameter block of 1 KiB instead of 11
 constexpr int kCtasPerSm = 4;
 constexpr int kMaxGrid = 1024;  // workspace slots of one launch
 
@@ -39,10 +40,11 @@ struct GradDesc {
   int8_t out_vec;  // `out` has 16-byte boundaries at the same elements
 };
 
+template <int kMax>
 struct GradArgs {
   int num;
-  int tile_start[kMaxTensors + 1];
-  GradDesc d[kMaxTensors];
+  int tile_start[kMax + 1];
+  GradDesc d[kMax];
 };
 
 // The raw bits of a thread's units of a tile; elements outside the tensor are 0.  Unit u holds elements
@@ -134,7 +136,8 @@ __device__ __forceinline__ double block_sum(double v) {
   return total;
 }
 
-__device__ __forceinline__ int64_t first_of(const GradArgs& args, int t, int tile) {
+template <int kMax>
+__device__ __forceinline__ int64_t first_of(const GradArgs<kMax>& args, int t, int tile) {
   return static_cast<int64_t>(tile - args.tile_start[t]) * kTileElems - args.d[t].shift + threadIdx.x * kUnit;
 }
 
@@ -171,7 +174,8 @@ __device__ __forceinline__ double tile_squares(const GradDesc& d, int64_t first)
   return sum;
 }
 
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) sum_squares_kernel(const __grid_constant__ GradArgs args, double* __restrict__ partials) {
+template <int kMax>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) sum_squares_kernel(const __grid_constant__ GradArgs<kMax> args, double* __restrict__ partials) {
   let_dependents_start();
   double sum = 0.0;
   const int tiles = args.tile_start[args.num];
@@ -221,7 +225,8 @@ __device__ __forceinline__ void clip_tile(const GradDesc& d, int64_t first, floa
   }
 }
 
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_kernel(const __grid_constant__ GradArgs args, const double* __restrict__ sums,
+template <int kMax>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_kernel(const __grid_constant__ GradArgs<kMax> args, const double* __restrict__ sums,
                                                                     int num_sums, float max_norm, float* __restrict__ norm) {
   grid_dependency_wait();
   const double n = sqrt(total_of(sums, num_sums));
@@ -295,10 +300,11 @@ int check_overlap(const fp8gmm_grad_desc* descs, int count, const char* name) {
 }
 
 // Fills `args` with the next descriptors, as many as one launch takes; returns the index of the first one left.
-int fill(GradArgs& args, const fp8gmm_grad_desc* descs, int i, int count) {
+template <int kMax>
+int fill(GradArgs<kMax>& args, const fp8gmm_grad_desc* descs, int i, int count) {
   args.num = 0;
   args.tile_start[0] = 0;
-  for (; i < count && args.num < kMaxTensors; ++i) {
+  for (; i < count && args.num < kMax; ++i) {
     const fp8gmm_grad_desc& t = descs[i];
     if (t.numel == 0) continue;
     const int size = static_cast<int>(elem_size(t.in_type));
@@ -315,21 +321,23 @@ int fill(GradArgs& args, const fp8gmm_grad_desc* descs, int i, int count) {
   return i;
 }
 
-int grid_of(const GradArgs& args) {
+template <int kMax>
+int grid_of(const GradArgs<kMax>& args) {
   const int cap = std::min(kMaxGrid, sm_count() * kCtasPerSm);
   return std::min(args.tile_start[args.num], cap);
 }
 
 // Partial sums of squares of all tensors into `partials`; *used = number of slots written.
+template <int kMax>
 int launch_sum_squares(const fp8gmm_grad_desc* descs, int count, double* partials, int slots, int* used, cudaStream_t s) {
-  GradArgs args;
+  GradArgs<kMax> args;
   *used = 0;
   for (int i = 0; i < count;) {
     i = fill(args, descs, i, count);
     if (args.num == 0) continue;
     const int grid = grid_of(args);
     FP8GMM_CHECK_ARG(*used + grid <= slots, "sum_squares: workspace too small");
-    sum_squares_kernel<<<grid, kThreads, 0, s>>>(args, partials + *used);
+    sum_squares_kernel<kMax><<<grid, kThreads, 0, s>>>(args, partials + *used);
     FP8GMM_CHECK_CUDA(cudaGetLastError());
     count_launch();
     *used += grid;
@@ -337,14 +345,15 @@ int launch_sum_squares(const fp8gmm_grad_desc* descs, int count, double* partial
   return FP8GMM_OK;
 }
 
+template <int kMax>
 int launch_clip(const fp8gmm_grad_desc* descs, int count, const double* sums, int num_sums, float max_norm, float* norm, bool after_sums, cudaStream_t s) {
-  GradArgs args;
+  GradArgs<kMax> args;
   for (int i = 0; i < count;) {
     i = fill(args, descs, i, count);
     if (args.num == 0) continue;
     // the first launch may follow the sums directly; a later one writes what the one before it may not have read yet only if
     // an entry's output were another's input, which is refused
-    FP8GMM_CHECK_CUDA(launch_dependent(clip_kernel, grid_of(args), kThreads, 0, s, after_sums, args, sums, num_sums, max_norm, norm));
+    FP8GMM_CHECK_CUDA(launch_dependent(clip_kernel<kMax>, grid_of(args), kThreads, 0, s, after_sums, args, sums, num_sums, max_norm, norm));
     count_launch();
     after_sums = false;
     norm = nullptr;
@@ -354,6 +363,18 @@ int launch_clip(const fp8gmm_grad_desc* descs, int count, const double* sums, in
     count_launch();
   }
   return FP8GMM_OK;
+}
+
+int launch_sum_squares(const fp8gmm_grad_desc* descs, int count, void* workspace, size_t bytes, int* used, cudaStream_t s) {
+  double* partials = static_cast<double*>(workspace);
+  const int slots = static_cast<int>(bytes / sizeof(double));
+  return count <= kFewTensors ? launch_sum_squares<kFewTensors>(descs, count, partials, slots, used, s)
+                              : launch_sum_squares<kMaxTensors>(descs, count, partials, slots, used, s);
+}
+int launch_clip(const fp8gmm_grad_desc* descs, int count, const double* sums, int num_sums, float max_norm, float* norm, bool after_sums,
+                cudaStream_t s) {
+  return count <= kFewTensors ? launch_clip<kFewTensors>(descs, count, sums, num_sums, max_norm, norm, after_sums, s)
+                              : launch_clip<kMaxTensors>(descs, count, sums, num_sums, max_norm, norm, after_sums, s);
 }
 
 int check_workspace(const void* workspace, size_t bytes, int count, const char* name) {
@@ -383,7 +404,7 @@ int fp8gmm_multi_sum_squares(const fp8gmm_grad_desc* descs, int count, void* wor
   if (rc != FP8GMM_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int used = 0;
-  rc = launch_sum_squares(descs, count, static_cast<double*>(workspace), static_cast<int>(workspace_bytes / sizeof(double)), &used, s);
+  rc = launch_sum_squares(descs, count, workspace, workspace_bytes, &used, s);
   if (rc != FP8GMM_OK) return rc;
   FP8GMM_CHECK_CUDA(launch_dependent(norm_kernel, 1, kThreads, 0, s, used > 0, static_cast<const double*>(workspace), used, sum, norm));
   count_launch();
@@ -413,7 +434,7 @@ int fp8gmm_multi_clip_grad_norm(const fp8gmm_grad_desc* descs, int count, float 
   if (rc != FP8GMM_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int used = 0;
-  rc = launch_sum_squares(descs, count, static_cast<double*>(workspace), static_cast<int>(workspace_bytes / sizeof(double)), &used, s);
+  rc = launch_sum_squares(descs, count, workspace, workspace_bytes, &used, s);
   if (rc != FP8GMM_OK) return rc;
   return launch_clip(descs, count, static_cast<const double*>(workspace), used, max_norm, norm, used > 0, s);
 }

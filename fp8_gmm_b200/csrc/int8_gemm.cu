@@ -9,14 +9,16 @@
 // The operands are swapped against gemm_sm100.cu: output channels are the M dimension of the MMA (TMEM lanes), rows the N
 // dimension (TMEM columns).  A group of any number of rows then costs an MMA only as wide as its rows, and a warp's 32 lanes
 // hold 32 neighbouring channels of one output row.
-// Two kernels:
-//   * int8_pair_kernel (many rows per group, tensor bound): persistent CTA pairs, tiles of 256 channels x up to 256 rows,
-//     accumulators double-buffered in TMEM, results transposed through shared memory and written as 256-byte runs;
-//   * int8_stream_kernel (few rows per group, bound by reading the weights): one tile of 128 channels x kT rows per CTA, the
-//     contraction optionally split over a cluster whose CTAs add their partial sums through distributed shared memory.
+//   * Persistent CTA pairs (cta_group::2): a tile is 256 channels x up to 64, 128 or 256 rows; each CTA loads its 128 channels
+//     of weights and half of the tile's rows; ring of 6 (256 rows) to 9 (64 rows) stages of 128 contraction bytes, accumulators
+//     double-buffered in TMEM, results transposed through shared memory and written as 256-byte runs.
+//   * The tiles that fill whole waves of the grid go to the pairs one after another; with few rows those of the last, partial wave
+//     are cut along the contraction so that every pair gets an equal share.  A pair that did a part of a tile leaves its sums in a workspace
+//     and counts itself in; the last one to come adds all parts up (integers: any order gives the same bits) and finishes the
+//     tile.  Nobody waits for anybody.
 // Group sizes come from the host (parameter block) or are read on the device; either way every CTA builds the prefix sums of
 // rows and tiles in shared memory.  Waits on mbarriers are bounded as in gemm_sm100.cu.
-#include <cstdlib>
+#include <atomic>
 #include <cstring>
 
 #include "int8.cuh"
@@ -34,35 +36,29 @@ constexpr int kWBytes = kChannels * kBlockK;
 
 struct Int8GemmParams {
   CUtensorMap map_w;                     // weights (G*N, K), box 128 rows x 128 bytes
-  CUtensorMap map_x;                     // codes (rows, K), box of the tile's rows (per CTA) x 128 bytes
+  CUtensorMap map_x;                     // codes (rows, K), box of half a tile's rows x 128 bytes
   uint16_t* c;
   const float* a_scales;
   const float* b_scales;
   const int64_t* device_sizes;           // group sizes on the device, or NULL: row_start holds their prefix sums
+  unsigned int* counters;                // workspace: parts that have come per split tile and CTA of the pair, zeroed
+  int* parts;                            // workspace: sums of parts, [pair][CTA][first, last][row][channel]; NULL = no splitting
   int* status;
   unsigned long long wait_ns;
   int num_groups, rows, n, k;
   int tile_rows, tiles_n, super_tiles;
+  int stages, stage_bytes;
   int row_start[kMaxGroups + 1];
 };
 
-// D[tmem] (+)= W[smem] X[smem]^T in 8-bit integers, issued by one thread.
-template <int kCtas>
-__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_w, uint64_t desc_x, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (kCtas == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_w), "l"(desc_x), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_w), "l"(desc_x), "r"(idesc), "r"(accumulate)
-        : "memory");
+// D[tmem] (+)= W[smem] X[smem]^T in 8-bit integers over both CTAs of the pair, issued by one thread of the leader.
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_w, uint64_t desc_x, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_w), "l"(desc_x), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 // Instruction descriptor of kind::i8: [4,6) D format (2 = s32), [7,10) / [10,13) A / B format (1 = signed), [17,23) N >> 3,
 // [24,29) M >> 4; both operands K-major.
@@ -70,27 +66,11 @@ __device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
-  uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
-  return r;
-}
-__device__ __forceinline__ void st_cluster32(uint32_t cluster_addr, uint32_t v) {
-  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_shared32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
 }
 
 __device__ __forceinline__ uint16_t result_bf16(uint32_t acc, float scale) {
@@ -150,7 +130,7 @@ struct Tile {
 };
 // Tiles of a group: super-rows of `super_tiles` row tiles, row tiles fastest inside one, so that the tiles in flight share
 // weights and codes through L2.
-__device__ __forceinline__ Tile decode_tile(const Int8GemmParams& p, const int* row_start, const int* tile_start, int tile, int channels) {
+__device__ __forceinline__ Tile decode_tile(const Int8GemmParams& p, const int* row_start, const int* tile_start, int tile) {
   Tile t;
   const int g = upper_slot(tile_start, p.num_groups, tile);
   const int local = tile - tile_start[g], m = row_start[g + 1] - row_start[g];
@@ -160,255 +140,99 @@ __device__ __forceinline__ Tile decode_tile(const Int8GemmParams& p, const int* 
   const int h = min(p.super_tiles, row_tiles - s * p.super_tiles);
   const int mt = s * p.super_tiles + rem % h;
   t.group = g;
-  t.n0 = rem / h * channels;
+  t.n0 = rem / h * (2 * kChannels);
   t.row0 = row_start[g] + mt * p.tile_rows;
   t.rows = min(p.tile_rows, m - mt * p.tile_rows);
   return t;
 }
 
-// =============================================================================================
-// Few rows per group: one tile of 128 channels x kT rows per CTA
-// =============================================================================================
-template <int kT>
-struct StreamCfg {
-  static constexpr int kXBytes = kT * kBlockK;
-  static constexpr int kStageBytes = kWBytes + kXBytes;
-  // two CTAs per SM, so that one streams weights while the other starts or ends: at most 110 KiB each
-  static constexpr int kStages = 108 * 1024 / kStageBytes;
-  static constexpr int kTmemCols = kT < 32 ? 32 : kT;
-  static constexpr int kTableBytes = 2 * (kMaxGroups + 1) * 4;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+// The work of one pair: whole tiles of the full waves, then its share of the last wave.
+struct Item {
+  int tile, kb0, kb1;
+  int rest;   // number of the tile in the last wave if that is split, else -1
+};
+struct Schedule {
+  int workers, worker, num_kb, full, rest, sharers, units;   // units: K blocks of the last wave
+  int i, u, u_end;
+
+  __device__ __forceinline__ Schedule(int worker_, int workers_, int total_tiles, int num_kb_, bool may_split)
+      : workers(workers_), worker(worker_), num_kb(num_kb_), full(total_tiles / workers_), rest(total_tiles - full * workers_), sharers(0),
+        units(rest * num_kb_), i(0), u(0), u_end(0) {
+    const int most = min(workers, units / kMinShare);
+    if (may_split && most > 0 && num_kb - (units + most - 1) / most >= kMinGain) {
+      sharers = most;
+      if (worker < sharers) {
+        u = begin_of(worker);
+        u_end = begin_of(worker + 1);
+      }
+    }
+  }
+  // The parts' way through L2 takes about 5 us, as long as 14 K blocks of weights: splitting has to save more.  (Measured with one
+  // row: 8 tiles of 56 K blocks 23.0 -> 13.2 us, 32 tiles of 112 41.4 -> 30.5, 32 tiles of 32 16.6 -> 16.9; with 54 tiles of 32 in
+  // the last wave, 9 K blocks to save, 29.5 -> 31.9.)
+  static constexpr int kMinGain = 16;
+  static constexpr int kMinShare = 8;
+  __device__ __forceinline__ int begin_of(int w) const { return static_cast<int>(static_cast<long long>(units) * w / sharers); }
+  // The pair whose share holds unit `at`.
+  __device__ __forceinline__ int sharer_of(int at) const {
+    return static_cast<int>((static_cast<long long>(at + 1) * sharers - 1) / units);
+  }
+  __device__ __forceinline__ bool next(Item& it) {
+    it.kb0 = 0;
+    it.kb1 = num_kb;
+    it.rest = -1;
+    if (i < full || (i == full && sharers == 0 && worker < rest)) {
+      it.tile = worker + i * workers;
+      ++i;
+      return true;
+    }
+    if (u >= u_end) return false;
+    it.rest = u / num_kb;
+    it.tile = full * workers + it.rest;
+    it.kb0 = u - it.rest * num_kb;
+    it.kb1 = min(num_kb, it.kb0 + u_end - u);
+    u += it.kb1 - it.kb0;
+    return true;
+  }
 };
 
-template <int kT>
-__global__ void __launch_bounds__(kThreads, 2) int8_stream_kernel(const __grid_constant__ Int8GemmParams p, int splits) {
-  using C = StreamCfg<kT>;
-  constexpr int kStages = C::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
-  uint8_t* tiles_ptr = smem_raw + (tiles_addr - raw_addr);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles_ptr + kStages * C::kStageBytes);
-  const uint32_t bar0 = smem_u32(bars);
-  auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
-  const uint32_t done_bar = bar0 + 8u * (2 * kStages);
-  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
-  // the group table is needed for the decoding alone: it lies in the first stage, before any load goes there
-  int* row_start = reinterpret_cast<int*>(tiles_ptr);
-  int* tile_start = row_start + kMaxGroups + 1;
-  static_assert(C::kTableBytes <= C::kStageBytes, "the group table has to fit into a stage");
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  if (threadIdx.x == 32) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
-    }
-    mbar_init(done_bar, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    prefetch_tensormap(&p.map_w);
-    prefetch_tensormap(&p.map_x);
-  }
-  if (warp == 2) {
-    tmem_alloc(smem_u32(tmem_base_slot), C::kTmemCols);
-    tmem_relinquish();
-  }
-  if (warp == 0) build_groups(p, row_start, tile_start, lane);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_base_slot;
-  const int tile = blockIdx.x / splits;
-  const bool live = tile < tile_start[p.num_groups];      // the same for all CTAs of a cluster
-  Tile t = {0, 0, 0, 0};
-  if (live) t = decode_tile(p, row_start, tile_start, tile, kChannels);
-  const int num_kb = (p.k + kBlockK - 1) / kBlockK;
-  const int kb0 = num_kb * rank / splits, kb1 = live ? num_kb * (rank + 1) / splits : kb0;
-  __syncthreads();                                        // everybody has read the table: loads may overwrite it
-  bool ok = true;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      fence_async_smem();   // the table's generic-proxy writes come before the loads into the same memory
-      const int yw = t.group * p.n + t.n0, first = min(kb1 - kb0, kStages);
-      // weights do not depend on the kernel before this one (the quantisation of the rows): their first loads go ahead of it
-      for (int i = 0; i < first; ++i) {
-        mbar_expect_tx(full_bar(i), C::kStageBytes);
-        tma_load_2d(tiles_addr + i * C::kStageBytes, &p.map_w, full_bar(i), (kb0 + i) * kBlockK, yw);
-      }
-      grid_dependency_wait();
-      for (int i = 0; i < first; ++i)
-        tma_load_2d(tiles_addr + i * C::kStageBytes + kWBytes, &p.map_x, full_bar(i), (kb0 + i) * kBlockK, t.row0);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0 + first; kb < kb1 && ok; ++kb) {
-        ok = mbar_wait(empty_bar(stage), phase, abort_flag, p.status, 0x1, p.wait_ns);
-        if (ok) {
-          const uint32_t sw = tiles_addr + stage * C::kStageBytes;
-          mbar_expect_tx(full_bar(stage), C::kStageBytes);
-          tma_load_2d(sw, &p.map_w, full_bar(stage), kb * kBlockK, yw);
-          tma_load_2d(sw + kWBytes, &p.map_x, full_bar(stage), kb * kBlockK, t.row0);
-        }
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0 && live) {
-      const uint32_t idesc = idesc_i8(kChannels, kT);
-      const uint64_t desc_w0 = make_smem_desc(tiles_addr), desc_x0 = make_smem_desc(tiles_addr + kWBytes);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, 0x4, p.wait_ns);
-        if (!ok) break;
-        const uint64_t dw = desc_w0 + static_cast<uint64_t>(stage * (C::kStageBytes >> 4));
-        const uint64_t dx = desc_x0 + static_cast<uint64_t>(stage * (C::kStageBytes >> 4));
-#pragma unroll
-        for (int k = 0; k < kBlockK / 32; ++k) umma_i8<1>(tmem_base, dw + 2 * k, dx + 2 * k, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
-        umma_commit(empty_bar(stage));
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (ok) umma_commit(done_bar);
-    }
-    __syncwarp();
-  }
-
-  const int quad = warp & 3;
-  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-  const int channel = t.n0 + quad * 32 + lane;
-  const bool epilogue = warp >= 2 && live;
-  const bool col_ok = channel < p.n;
-  float sb = 0.f;
-  if (epilogue) {
-    grid_dependency_wait();
-    if (col_ok) sb = p.b_scales[static_cast<int64_t>(t.group) * p.n + channel];
-    if (lane == 0) ok = mbar_wait(done_bar, 0, abort_flag, p.status, 0x8, p.wait_ns);
-    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-    tc_fence_after();
-  }
-  uint16_t* dst = p.c + static_cast<int64_t>(t.row0) * p.n + channel;
-  if (splits == 1) {
-    if (epilogue && ok) {
-#pragma unroll
-      for (int c0 = 0; c0 < kT; c0 += 16) {
-        if (c0 >= t.rows) break;
-        const float my_sa = lane < 16 && c0 + lane < t.rows ? p.a_scales[t.row0 + c0 + lane] : 0.f;
-        uint32_t r[16];
-        tmem_ld16(taddr + c0, r);
-        tc_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float s = __fmul_rn(__shfl_sync(0xFFFFFFFFu, my_sa, j), sb);
-          if (col_ok && c0 + j < t.rows) dst[static_cast<int64_t>(c0 + j) * p.n] = result_bf16(r[j], s);
-        }
-      }
-    }
-  } else {
-    // Each CTA of the cluster finishes kT / splits of the rows: it receives the other CTAs' partial sums of them in its (now
-    // idle) stages, [sender][row][channel].
-    const int width = kT / splits;
-    __syncwarp();
-    cluster_sync_all();
-    if (epilogue && ok) {
-#pragma unroll
-      for (int c0 = 0; c0 < kT; c0 += 16) {
-        uint32_t r[16];
-        tmem_ld16(taddr + c0, r);
-        tc_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int to = (c0 + j) / width, row = c0 + j - to * width;
-          if (to != rank) {
-            const int slot = rank < to ? rank : rank - 1;
-            const uint32_t at = tiles_addr + static_cast<uint32_t>(((slot * width + row) * kChannels + quad * 32 + lane) * 4);
-            st_cluster32(map_to_cta(at, static_cast<uint32_t>(to)), r[j]);
-          }
-        }
-      }
-    }
-    __syncwarp();
-    cluster_sync_all();
-    if (epilogue && ok) {
-      for (int row = 0; row < width; ++row) {
-        const int token = rank * width + row;
-        if (token >= t.rows) break;
-        uint32_t acc = tmem_ld1(taddr + token);
-        tc_wait_ld();
-        for (int slot = 0; slot < splits - 1; ++slot)
-          acc += ld_shared32(tiles_addr + static_cast<uint32_t>(((slot * width + row) * kChannels + quad * 32 + lane) * 4));
-        const float s = __fmul_rn(p.a_scales[t.row0 + token], sb);
-        if (col_ok) dst[static_cast<int64_t>(token) * p.n] = result_bf16(acc, s);
-      }
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag) {  // copies and MMAs still in flight get time to land before shared memory and TMEM go away
-    const unsigned long long t0 = global_ns();
-    while (global_ns() - t0 < 200000ull) {
-    }
-  }
-  __syncthreads();
-  if (warp == 2) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, C::kTmemCols);
-  }
-}
-
-// =============================================================================================
-// Many rows per group: persistent CTA pairs, 256 channels x up to 256 rows per tile
-// =============================================================================================
-struct PairCfg {
-  static constexpr int kRows = 256;
-  static constexpr int kStages = 6;
-  static constexpr int kStageBytes = kWBytes + kRows / 2 * kBlockK;   // 32 KiB per CTA
-  static constexpr int kTmemCols = 512;
-  static constexpr int kStagingBytes = 2 * 32 * kChannels * 2;        // two boxes of 32 rows x 128 channels of bf16
-  static constexpr int kScaleBytes = 2 * kRows * 4;
-  static constexpr int kTableBytes = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kScaleBytes + kTableBytes + 1024 + 256;
-};
+constexpr int kMinRows = 64, kMaxRows = 256;  // rows of the smallest and the largest tile
+constexpr int kMaxStages = 9;
+constexpr int kRingBytes = 6 * 32 * 1024;
+constexpr int kTmemCols = 512;
+constexpr int kBoxBytes = 32 * kChannels * 2; // 32 rows x 128 channels of bf16
+constexpr int kStagingBytes = 2 * kBoxBytes;
+constexpr int kScaleBytes = 2 * kMaxRows * 4;
+constexpr int kTableBytes = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
+constexpr int kSmemBytes = kRingBytes + kStagingBytes + kScaleBytes + kTableBytes + 1024 + 256;
 
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_constant__ Int8GemmParams p) {
-  using C = PairCfg;
-  constexpr int kStages = C::kStages;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_constant__ Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
-  uint8_t* staging = smem_raw + (tiles_addr - raw_addr) + kStages * C::kStageBytes;
-  float* scale_buf = reinterpret_cast<float*>(staging + C::kStagingBytes);
-  int* row_start = reinterpret_cast<int*>(staging + C::kStagingBytes + C::kScaleBytes);
+  uint8_t* staging = smem_raw + (tiles_addr - raw_addr) + kRingBytes;
+  float* scale_buf = reinterpret_cast<float*>(staging + kStagingBytes);
+  int* row_start = reinterpret_cast<int*>(staging + kStagingBytes + kScaleBytes);
   int* tile_start = row_start + kMaxGroups + 1;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes + C::kScaleBytes + C::kTableBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStagingBytes + kScaleBytes + kTableBytes);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
-  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * kStages + a); };
-  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
-  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + a); };
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 2 + a); };
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+  volatile int* finish_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const bool leader = rank == 0;
-  const int worker = blockIdx.x >> 1, num_workers = gridDim.x >> 1;
+  const int stages = p.stages, stage_bytes = p.stage_bytes;
 
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
@@ -423,37 +247,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_pa
     prefetch_tensormap(&p.map_x);
   }
   if (warp == 2) {
-    tmem_alloc_pair(smem_u32(tmem_base_slot), C::kTmemCols);
+    tmem_alloc_pair(smem_u32(tmem_base_slot), kTmemCols);
     tmem_relinquish_pair();
   }
   if (warp == 0) build_groups(p, row_start, tile_start, lane);
   tc_fence_before();
   cluster_sync_all();
   tc_fence_after();
-  grid_dependency_wait();
   const uint32_t tmem_base = *tmem_base_slot;
-  const int total_tiles = tile_start[p.num_groups];
-  const int num_kb = (p.k + kBlockK - 1) / kBlockK;
+  Schedule work(blockIdx.x >> 1, gridDim.x >> 1, tile_start[p.num_groups], (p.k + kBlockK - 1) / kBlockK, p.parts != nullptr);
+  Item it;
 
   if (warp == 0) {
+    // ===================== TMA producer: both CTAs credit the leader's barriers =====================
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      bool ok = true;
+      bool ok = true, waited = false;
       const uint32_t full0_leader = map_to_cta(full_bar(0), 0);
-      for (int tile = worker; tile < total_tiles && ok; tile += num_workers) {
-        const Tile t = decode_tile(p, row_start, tile_start, tile, 2 * kChannels);
+      while (ok && work.next(it)) {
+        const Tile t = decode_tile(p, row_start, tile_start, it.tile);
         const int width = (t.rows + 31) & ~31;                       // columns of this tile's MMAs, half of them from each CTA
         const int yw = t.group * p.n + t.n0 + rank * kChannels, yx = t.row0 + rank * (width / 2);
-        for (int kb = 0; kb < num_kb && ok; ++kb) {
+        int kb = it.kb0;
+        if (!waited) {
+          // Weights do not depend on the kernel before this one (the quantisation of the rows): a ring full of them goes ahead.
+          waited = true;
+          const int first = min(it.kb1 - it.kb0, stages);
+          for (int i = 0; i < first; ++i) {
+            if (leader) mbar_expect_tx(full_bar(i), 2 * stage_bytes);
+            tma_load_2d_pair(tiles_addr + i * stage_bytes, &p.map_w, full0_leader + 8u * i, (kb + i) * kBlockK, yw);
+          }
+          grid_dependency_wait();
+          for (int i = 0; i < first; ++i)
+            tma_load_2d_pair(tiles_addr + i * stage_bytes + kWBytes, &p.map_x, full0_leader + 8u * i, (kb + i) * kBlockK, yx);
+          kb += first;
+          stage = first == stages ? 0 : first;
+          phase = first == stages ? 1u : 0u;
+        }
+        for (; kb < it.kb1 && ok; ++kb) {
           ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x1, p.wait_ns);
           if (ok) {
-            const uint32_t sw = tiles_addr + stage * C::kStageBytes, bar = full0_leader + 8u * stage;
-            if (leader) mbar_expect_tx(full_bar(stage), 2 * C::kStageBytes);   // both CTAs credit the leader's barrier
+            const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
+            if (leader) mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
             tma_load_2d_pair(sw, &p.map_w, bar, kb * kBlockK, yw);
             tma_load_2d_pair(sw + kWBytes, &p.map_x, bar, kb * kBlockK, yx);
           }
-          if (++stage == kStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -462,27 +302,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_pa
     }
     __syncwarp();
   } else if (warp == 1) {
+    // ===================== MMA issuer: one thread of the leader =====================
     if (leader && lane == 0) {
       const uint64_t desc_w0 = make_smem_desc(tiles_addr), desc_x0 = make_smem_desc(tiles_addr + kWBytes);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = worker; tile < total_tiles && ok; tile += num_workers) {
-        const Tile t = decode_tile(p, row_start, tile_start, tile, 2 * kChannels);
+      while (ok && work.next(it)) {
+        const Tile t = decode_tile(p, row_start, tile_start, it.tile);
         const uint32_t idesc = idesc_i8(2 * kChannels, (t.rows + 31) & ~31);
         ok = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.status, 0x2, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * C::kRows);
-        for (int kb = 0; kb < num_kb; ++kb) {
+        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kMaxRows);
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
           ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, 0x4, p.wait_ns);
           if (!ok) break;
-          const uint64_t dw = desc_w0 + static_cast<uint64_t>(stage * (C::kStageBytes >> 4));
-          const uint64_t dx = desc_x0 + static_cast<uint64_t>(stage * (C::kStageBytes >> 4));
+          const uint64_t dw = desc_w0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
+          const uint64_t dx = desc_x0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k) umma_i8<2>(tmem_d, dw + 2 * k, dx + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          for (int k = 0; k < kBlockK / 32; ++k) umma_i8_pair(tmem_d, dw + 2 * k, dx + 2 * k, idesc, (kb != it.kb0 || k != 0) ? 1u : 0u);
           umma_commit_pair(empty_bar(stage));
-          if (++stage == kStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -495,62 +336,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_pa
     }
     __syncwarp();
   } else {
+    // ===================== epilogue: 128 threads, one channel each =====================
+    // A warp that gave up on a wait goes on through the barriers, which count all four.
     const int quad = warp & 3, thread = threadIdx.x - 64;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int tile = worker; tile < total_tiles; tile += num_workers) {
-      const Tile t = decode_tile(p, row_start, tile_start, tile, 2 * kChannels);
+    grid_dependency_wait();
+    while (work.next(it)) {
+      const Tile t = decode_tile(p, row_start, tile_start, it.tile);
       const int n0 = t.n0 + rank * kChannels;
       const int channel = n0 + quad * 32 + lane;
       const float sb = channel < p.n ? p.b_scales[static_cast<int64_t>(t.group) * p.n + channel] : 0.f;
-      float* scales = scale_buf + acc * C::kRows;
+      float* scales = scale_buf + acc * kMaxRows;
       for (int i = thread; i < t.rows; i += 128) scales[i] = p.a_scales[t.row0 + i];
       if (lane == 0 && ok) ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 0x8, p.wait_ns);
       ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-      epilogue_barrier();     // the scales are there; every warp goes on, also one that gave up, as the barriers count all four
+      epilogue_barrier();
       tc_fence_after();
-      const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * C::kRows) + (static_cast<uint32_t>(quad * 32) << 16);
-      for (int c0 = 0; c0 < t.rows; c0 += 32) {
-        uint16_t* box = reinterpret_cast<uint16_t*>(staging) + ((c0 >> 5) & 1) * 32 * kChannels;
+      const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * kMaxRows) + (static_cast<uint32_t>(quad * 32) << 16);
+
+      bool finish = true;
+      int first_sharer = 0, last_sharer = -1, tile_begin = 0;
+      const int64_t part_stride = static_cast<int64_t>(p.tile_rows) * kChannels;
+      if (it.rest >= 0 && it.kb1 - it.kb0 < work.num_kb) {
+        // Part of a tile: its sums go to the workspace, in the place of this pair's first or last tile.
+        tile_begin = it.rest * work.num_kb;
+        first_sharer = work.sharer_of(tile_begin);
+        last_sharer = work.sharer_of(tile_begin + work.num_kb - 1);
+        const int place = tile_begin + it.kb0 == work.begin_of(work.worker) ? 0 : 1;
+        const int rows8 = (t.rows + 7) & ~7;
         if (ok) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c0, r);
-          tc_wait_ld();
-          uint16_t* mine = box + quad * 32 + lane;
+          int* out = p.parts + ((static_cast<int64_t>(work.worker) * 2 + rank) * 2 + place) * part_stride + quad * 32 + lane;
+          for (int c0 = 0; c0 < rows8; c0 += 8) {
+            uint32_t r[8];
+            tmem_ld8(taddr + c0, r);
+            tc_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 sa = *reinterpret_cast<const float4*>(scales + c0 + j);
-            mine[(j + 0) * kChannels] = result_bf16(r[j + 0], __fmul_rn(sa.x, sb));
-            mine[(j + 1) * kChannels] = result_bf16(r[j + 1], __fmul_rn(sa.y, sb));
-            mine[(j + 2) * kChannels] = result_bf16(r[j + 2], __fmul_rn(sa.z, sb));
-            mine[(j + 3) * kChannels] = result_bf16(r[j + 3], __fmul_rn(sa.w, sb));
+            for (int j = 0; j < 8; ++j) __stcg(out + (c0 + j) * kChannels, static_cast<int>(r[j]));
           }
         }
         epilogue_barrier();
-        // 16 threads write the 256 bytes of a row; the box is free again after the next barrier
-        const int chunk = thread & 15;
-        if (ok && n0 + chunk * 8 < p.n) {
+        if (thread == 0) {
+          // behind the barrier this thread has seen the others' stores: its release covers them, its acquire what they read next
+          __threadfence();
+          const unsigned int before = atomicAdd(p.counters + it.rest * 2 + rank, 1u);
+          __threadfence();
+          *finish_flag = before == static_cast<unsigned int>(last_sharer - first_sharer);
+        }
+        epilogue_barrier();
+        finish = *finish_flag != 0;
+      }
+      if (finish) {
+        for (int c0 = 0; c0 < t.rows; c0 += 32) {
+          uint16_t* box = reinterpret_cast<uint16_t*>(staging + ((c0 >> 5) & 1) * kBoxBytes);
+          if (ok) {
+            uint32_t r[32];
+            tmem_ld32(taddr + c0, r);
+            tc_wait_ld();
+            if (last_sharer >= first_sharer) {
+              // the others' parts, eight rows of up to four of them in flight
 #pragma unroll
-          for (int it = 0; it < 4; ++it) {
-            const int row = it * 8 + (thread >> 4);
-            if (c0 + row < t.rows)
-              *reinterpret_cast<uint4*>(p.c + static_cast<int64_t>(t.row0 + c0 + row) * p.n + n0 + chunk * 8) =
-                  *reinterpret_cast<const uint4*>(box + row * kChannels + chunk * 8);
+              for (int j0 = 0; j0 < 32; j0 += 8) {
+                if (c0 + j0 >= t.rows) break;
+                for (int w0 = first_sharer; w0 <= last_sharer; w0 += 4) {
+                  int other[4][8];
+#pragma unroll
+                  for (int v = 0; v < 4; ++v) {
+                    const int w = w0 + v;
+                    const bool there = w <= last_sharer && w != work.worker;
+                    const int place = there && work.begin_of(w) >= tile_begin ? 0 : 1;
+                    const int* in = p.parts + ((static_cast<int64_t>(w) * 2 + rank) * 2 + place) * part_stride + quad * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) other[v][j] = there ? __ldcg(in + (c0 + j0 + j) * kChannels) : 0;
+                  }
+#pragma unroll
+                  for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[j0 + j] += static_cast<uint32_t>(other[v][j]);
+                }
+              }
+            }
+            uint16_t* mine = reinterpret_cast<uint16_t*>(box) + quad * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 sa = *reinterpret_cast<const float4*>(scales + c0 + j);
+              mine[(j + 0) * kChannels] = result_bf16(r[j + 0], __fmul_rn(sa.x, sb));
+              mine[(j + 1) * kChannels] = result_bf16(r[j + 1], __fmul_rn(sa.y, sb));
+              mine[(j + 2) * kChannels] = result_bf16(r[j + 2], __fmul_rn(sa.z, sb));
+              mine[(j + 3) * kChannels] = result_bf16(r[j + 3], __fmul_rn(sa.w, sb));
+            }
+          }
+          epilogue_barrier();
+          // 16 threads write the 256 bytes of a row; the box is free again after the next barrier
+          const int chunk = thread & 15;
+          if (ok && n0 + chunk * 8 < p.n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = i * 8 + (thread >> 4);
+              if (c0 + row < t.rows)
+                *reinterpret_cast<uint4*>(p.c + static_cast<int64_t>(t.row0 + c0 + row) * p.n + n0 + chunk * 8) =
+                    *reinterpret_cast<const uint4*>(box + row * kChannels + chunk * 8);
+            }
           }
         }
       }
-      epilogue_barrier();     // the last box is read before the next tile writes into it
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(map_to_cta(tempty_bar(acc), 0));
+      epilogue_barrier();     // the last box and the flag are read before the next tile writes them
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
   }
   tc_fence_before();
   cluster_sync_all();
-  if (*abort_flag) {
+  if (*abort_flag) {  // copies and MMAs still in flight get time to land before shared memory and TMEM go away
     const unsigned long long t0 = global_ns();
     while (global_ns() - t0 < 200000ull) {
     }
@@ -558,7 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_pa
   cluster_sync_all();   // a CTA must not leave while its peer can still touch its shared memory or barriers
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, C::kTmemCols);
+    tmem_dealloc_pair(tmem_base, kTmemCols);
   }
 }
 
@@ -587,42 +488,53 @@ int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, 
 }
 
 // Process-wide override for tests (fp8gmm_set_int8_variant): 0 = chosen per call.
-int g_tile_rows = 0, g_splits = 0;
+int g_tile_rows = 0;
+int g_split = 1;
 
-template <typename... Args>
-int launch(void (*kernel)(Args...), int grid, int cluster, int smem, cudaStream_t s, bool early, Args... args) {
-  FP8GMM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  if (early) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  if (cluster > 1) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = cluster;
-    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  cfg.attrs = attr;
-  FP8GMM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-  count_launch();
+constexpr int kCounterBytes = 1024;   // two counters for each tile of a partial wave (fewer tiles than pairs)
+
+// Once per device: the attribute stays.
+int allow_shared_memory() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  FP8GMM_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit) != 0) return FP8GMM_OK;
+  FP8GMM_CHECK_CUDA(cudaFuncSetAttribute(int8_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
   return FP8GMM_OK;
 }
 
-template <int kT>
-int launch_stream(Int8GemmParams& p, int64_t row_tiles, int splits, cudaStream_t s, bool early) {
-  const int64_t grid = row_tiles * p.tiles_n * splits;
-  FP8GMM_CHECK_ARG(grid <= INT32_MAX, "int8_grouped_gemm: problem too large");
-  return launch<Int8GemmParams, int>(int8_stream_kernel<kT>, static_cast<int>(grid), splits, StreamCfg<kT>::kSmemBytes, s, early, p, splits);
+int pairs() { return sm_count() / 2; }
+
+// Rows of a tile.  Few rows per group: smaller tiles leave more stages for weights in flight and compute less on empty columns
+// (20 GB/s of weights per SM more with 64 than with 256); many: larger ones read the weights less often.  Measured, product
+// and quantisation, us (64 / 128 / 256 rows): eight experts of 4096 x 4096 with 8 rows each 29.5 / 29.8 / 29.8, with 32 rows
+// 34.2 / 32.0 / 32.6, with 128 rows 62.6 / 47.9 / 40.7; 64 experts of 1424 x 2048 with 8 rows 38.6 / 38.7 / 40.0, with 64 rows
+// 64.1 / 53.6 / 54.7, with 256 rows 171 / 117 / 97.  A grid that would not be filled takes smaller tiles: one expert of
+// 1024 x 4096 with 1024 rows 21.0 / 21.6 / 22.7; 4096 x 14336 with 300 rows 78 (second wave) / 45.9 / 47.3.
+int choose_tile_rows(const fp8gmm_int8_gemm_args* a) {
+  if (g_tile_rows != 0) return g_tile_rows;
+  const int64_t tiles_n = (a->n + 2 * kChannels - 1) / (2 * kChannels);
+  const int64_t groups = a->rows < a->num_groups ? a->rows : a->num_groups;   // groups that can have rows
+  const int64_t mean = (a->rows + groups - 1) / groups;
+  int t = mean <= 16 ? 64 : mean <= 64 ? 128 : 256;
+  while (t > kMinRows && groups * ((mean + t / 2 - 1) / (t / 2)) * tiles_n <= pairs()) t /= 2;
+  return t;
+}
+
+// Bytes of workspace with which the tiles of a partial wave can be split; 0 where that does not pay: with larger tiles (the parts
+// of 128 rows cost more than the idle pairs: 300 rows, K = 14336: 54 us against 46), a short contraction or many waves.
+size_t workspace_bytes(const fp8gmm_int8_gemm_args* a, int tile_rows) {
+  if (a->rows <= 0 || a->num_groups <= 0 || g_split == 0 || tile_rows != kMinRows) return 0;
+  const int64_t groups = a->rows < a->num_groups ? a->rows : a->num_groups;
+  const int64_t tiles = (a->rows / tile_rows + groups) * ((a->n + 2 * kChannels - 1) / (2 * kChannels));
+  if (tiles > 8 * static_cast<int64_t>(pairs()) || a->k <= kBlockK * Schedule::kMinGain) return 0;
+  return kCounterBytes + static_cast<size_t>(pairs()) * 4 * tile_rows * kChannels * sizeof(int);
 }
 
 }  // namespace
+
 // Argument checks; nothing is launched and no CUDA call made.
 int int8_gemm_check(const fp8gmm_int8_gemm_args* a) {
   FP8GMM_CHECK_ARG(a != nullptr, "int8_grouped_gemm: NULL arguments");
@@ -646,6 +558,7 @@ int int8_gemm_check(const fp8gmm_int8_gemm_args* a) {
   FP8GMM_CHECK_ARG(a->a && a->b && a->c && a->a_scales && a->b_scales, "int8_grouped_gemm: NULL pointer");
   FP8GMM_CHECK_ARG((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->b) | reinterpret_cast<uintptr_t>(a->c)) % 16 == 0,
                    "int8_grouped_gemm: operand pointers must be 16-byte aligned");
+  FP8GMM_CHECK_ARG(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "int8_grouped_gemm: the workspace must be 16-byte aligned");
   return FP8GMM_OK;
 }
 
@@ -666,56 +579,54 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
   p.wait_ns = gemm_wait_limit_ns();
   p.status = device_status_word();
   FP8GMM_CHECK_ARG(p.status != nullptr, "int8_grouped_gemm: cannot resolve the device status word");
-  // The rule goes by the mean rows of a group that can have any, so that sizes on the host and on the device take the same path.
-  const int groups = p.rows < p.num_groups ? p.rows : p.num_groups;
-  const int mean = (p.rows + groups - 1) / groups;
-  int tile_rows = g_tile_rows;
-  if (tile_rows == 0) tile_rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+  const int tile_rows = choose_tile_rows(a);
   p.tile_rows = tile_rows;
   rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, kChannels);
   if (rc != FP8GMM_OK) return rc;
-  rc = encode_rows(&p.map_x, a->a, a->rows, a->k, tile_rows == 256 ? 128 : tile_rows);
+  rc = encode_rows(&p.map_x, a->a, a->rows, a->k, tile_rows / 2);
   if (rc != FP8GMM_OK) return rc;
+  p.stage_bytes = kWBytes + tile_rows / 2 * kBlockK;
+  p.stages = kRingBytes / p.stage_bytes < kMaxStages ? kRingBytes / p.stage_bytes : kMaxStages;
+  p.tiles_n = (p.n + 2 * kChannels - 1) / (2 * kChannels);
+  // a band of codes of 4096 rows (2048 with a long contraction) stays in L2 while the channel tiles sweep past it
+  p.super_tiles = (p.k > 8192 ? 2048 : 4096) / tile_rows;
   // each group adds at most one partial row tile to rows / tile_rows
-  const int64_t row_tiles = p.rows / tile_rows + groups;
-  const int channels = tile_rows == 256 ? 2 * kChannels : kChannels;
-  p.tiles_n = (p.n + channels - 1) / channels;
-  FP8GMM_CHECK_ARG(row_tiles * p.tiles_n <= INT32_MAX / 2, "int8_grouped_gemm: problem too large");
+  const int64_t most = (p.rows / tile_rows + (p.rows < p.num_groups ? p.rows : p.num_groups)) * static_cast<int64_t>(p.tiles_n);
+  FP8GMM_CHECK_ARG(most <= INT32_MAX / 2, "int8_grouped_gemm: problem too large");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (tile_rows == 256) {
-    p.super_tiles = (p.k > 8192 ? 2048 : 4096) / PairCfg::kRows;
-    int sms = sm_count() / 2;
-    const int64_t most = row_tiles * p.tiles_n;
-    return launch<Int8GemmParams>(int8_pair_kernel, 2 * static_cast<int>(most < sms ? most : sms), 1, PairCfg::kSmemBytes, s, after_quantize, p);
+  const size_t want = workspace_bytes(a, tile_rows);
+  int workers = pairs();
+  if (want > 0 && a->workspace != nullptr && a->workspace_bytes >= want) {
+    p.counters = static_cast<unsigned int*>(a->workspace);
+    p.parts = reinterpret_cast<int*>(static_cast<char*>(a->workspace) + kCounterBytes);
+    if (!after_quantize) FP8GMM_CHECK_CUDA(cudaMemsetAsync(p.counters, 0, kCounterBytes, s));
+  } else if (most < workers) {
+    workers = static_cast<int>(most);
   }
-  p.super_tiles = INT32_MAX / 2 / p.tiles_n;   // row tiles fastest: the CTAs that share weights run side by side
-  int splits = g_splits;
-  const int num_kb = (p.k + kBlockK - 1) / kBlockK;
-  if (splits == 0) {
-    splits = 1;
-    const int64_t tiles = row_tiles * p.tiles_n;
-    while (splits < 8 && tiles * splits < 2 * sm_count() && num_kb >= 8 * splits) splits *= 2;
-  }
-  while (splits > num_kb || splits > tile_rows) splits /= 2;
-  switch (tile_rows) {
-    case 16: return launch_stream<16>(p, row_tiles, splits, s, after_quantize);
-    case 32: return launch_stream<32>(p, row_tiles, splits, s, after_quantize);
-    case 64: return launch_stream<64>(p, row_tiles, splits, s, after_quantize);
-    default: return launch_stream<128>(p, row_tiles, splits, s, after_quantize);
-  }
+  rc = allow_shared_memory();
+  if (rc != FP8GMM_OK) return rc;
+  FP8GMM_CHECK_CUDA(launch_dependent(int8_gemm_kernel, 2 * workers, kThreads, kSmemBytes, s, after_quantize, p));
+  count_launch();
+  return FP8GMM_OK;
 }
+
 }  // namespace fp8gmm
 
 extern "C" {
 
-int fp8gmm_set_int8_variant(int tile_rows, int splits) {
+int fp8gmm_set_int8_variant(int tile_rows, int split) {
   using namespace fp8gmm;
-  FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 16 || tile_rows == 32 || tile_rows == 64 || tile_rows == 128 || tile_rows == 256,
-                   "set_int8_variant: tile_rows must be 0, 16, 32, 64, 128 or 256");
-  FP8GMM_CHECK_ARG(splits == 0 || splits == 1 || splits == 2 || splits == 4 || splits == 8, "set_int8_variant: splits must be 0, 1, 2, 4 or 8");
+  FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 64 || tile_rows == 128 || tile_rows == 256,
+                   "set_int8_variant: tile_rows must be 0, 64, 128 or 256");
   g_tile_rows = tile_rows;
-  g_splits = splits;
+  g_split = split != 0;
   return FP8GMM_OK;
+}
+
+size_t fp8gmm_int8_workspace_bytes(const fp8gmm_int8_gemm_args* a) {
+  using namespace fp8gmm;
+  if (a == nullptr || a->rows <= 0 || a->num_groups <= 0) return 0;
+  return workspace_bytes(a, choose_tile_rows(a));
 }
 
 int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) { return fp8gmm::int8_gemm_launch(a, stream, false); }
@@ -726,7 +637,8 @@ int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gem
                    "int8_linear: the product has to take the codes, scales, rows and columns of the quantisation");
   int rc = fp8gmm::int8_gemm_check(g);   // before anything is launched
   if (rc != FP8GMM_OK) return rc;
-  rc = fp8gmm_quantize_rows_int8(q, stream);
+  // the quantisation zeroes the counters that the product's split tiles need
+  rc = fp8gmm::quantize_rows_launch(q, g->workspace_bytes >= fp8gmm::kCounterBytes ? g->workspace : nullptr, fp8gmm::kCounterBytes / 4, stream);
   return rc != FP8GMM_OK ? rc : fp8gmm::int8_gemm_launch(g, stream, q->rows > 0);
 }
 

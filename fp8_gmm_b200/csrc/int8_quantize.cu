@@ -12,7 +12,7 @@
 // A row of zeros has scale 0 and codes 0.  A row that holds an infinity or a NaN has scale NaN and codes 0: all its products
 // come out NaN, no other row's do.
 //
-// Two kernels.  quantize_rows_kernel: one CTA per row, the row in registers between the maximum and the codes, so it is read
+// Two kernels.  quantize_rows_kernel: a block for one row or several short ones, the row in registers between the maximum and the codes, so it is read
 // once; 16-byte loads, 8-byte stores.  quantize_long_rows_kernel: rows that are too long for that, or not aligned to 16 bytes,
 // are walked twice (the second time out of L2 or L1).
 #include "int8.cuh"
@@ -21,8 +21,8 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kLongThreads = 256;
-constexpr int kMaxThreads = 512;
-constexpr int kMaxVecs = 4;              // 8-element vectors a thread holds: rows of up to 512 * 4 * 8 = 16384 elements
+constexpr int kMaxThreads = 1024;
+constexpr int kVecs = 2;                 // 8-element vectors a thread holds: rows of up to 1024 * 2 * 8 = 16384 elements
 constexpr int kStatusBadIndex = 0x200;   // as in routing.cu: an index that names no row
 
 struct QuantRowsParams {
@@ -35,6 +35,8 @@ struct QuantRowsParams {
   int8_t* codes;
   float* scales;
   int* status;
+  uint32_t* zero;      // words to be zeroed for the kernel behind this one, or NULL
+  int zero_words;
 };
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
@@ -71,16 +73,27 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
   }
   return s;
 }
-// The code in the low byte: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.
+// The code in the low byte: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.  Behind
+// an activation there are no exact ties to respect (v itself is rounded), and one fused multiply-add does it.
+template <int kAct>
 __device__ __forceinline__ uint32_t code_of(float v, const RowScale& s) {
+  constexpr float kMagic = 12582912.f;
+  if constexpr (kAct != FP8GMM_ACT_NONE) return __float_as_uint(fmaf(v, s.pre * s.inv, kMagic));
   const float t = v * s.pre;
   float y = t * s.inv;
   y = fmaf(fmaf(-y, s.top, t), s.inv, y);
-  return __float_as_uint(y + 12582912.f);
+  return __float_as_uint(y + kMagic);
+}
+// max(a, |b|), NaN if either is
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 
-// Maximum over the block; `warp_max` has a place for every warp.
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* warp_max) {
+// Maximum over the threads of one row (blockDim.x of them, whole warps) of bits of non-negative floats (ordered like them, NaN
+// above infinity); `warp_max` has a place for every warp of the row.
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* warp_max) {
   v = __reduce_max_sync(0xFFFFFFFFu, v);
   const int warps = blockDim.x >> 5;
   if (warps == 1) return v;
@@ -88,6 +101,11 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* warp_max) {
   __syncthreads();
   const int lane = threadIdx.x & 31;
   return __reduce_max_sync(0xFFFFFFFFu, lane < warps ? warp_max[lane] : 0u);
+}
+
+__device__ __forceinline__ void zero_words(const QuantRowsParams& p) {
+  if (p.zero != nullptr && blockIdx.x == 0 && threadIdx.y == 0)
+    for (int i = threadIdx.x; i < p.zero_words; i += blockDim.x) p.zero[i] = 0u;
 }
 
 // Source row of row r, or -1 (reported) if the index names none.
@@ -100,12 +118,14 @@ __device__ __forceinline__ int64_t source_row(const QuantRowsParams& p, int64_t 
   return -1;
 }
 
-template <int kAct, int kVecs>
-__global__ void __launch_bounds__(kMaxThreads) quantize_rows_kernel(const QuantRowsParams p) {
+template <int kAct>
+__global__ void __launch_bounds__(kMaxThreads, 2) quantize_rows_kernel(const QuantRowsParams p) {
   __shared__ uint32_t warp_max[kMaxThreads / 32];
   let_dependents_start();
-  const int64_t r = blockIdx.x;
-  const int64_t src = source_row(p, r);
+  zero_words(p);
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const bool live = r < p.rows;
+  const int64_t src = live ? source_row(p, r) : -1;
   const int vecs = static_cast<int>(p.cols >> 3);
   const uint4* a = reinterpret_cast<const uint4*>(p.in + (src < 0 ? 0 : src) * p.in_ld);
   uint4 raw[kVecs], raw2[kAct == FP8GMM_ACT_SWIGLU ? kVecs : 1];
@@ -117,7 +137,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_rows_kernel(const QuantR
     if constexpr (kAct == FP8GMM_ACT_SWIGLU) raw2[u] = in ? __ldg(a + vecs + c) : make_uint4(0, 0, 0, 0);   // [gate | up]
   }
   float v[kVecs][8];
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
     const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
@@ -127,11 +147,11 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_rows_kernel(const QuantR
     for (int j = 0; j < 4; ++j) {
       v[u][2 * j] = activated<kAct>(bf16_lo(w[j]), bf16_lo(w2[j]));
       v[u][2 * j + 1] = activated<kAct>(bf16_hi(w[j]), bf16_hi(w2[j]));
-      // ordered as integers, with NaN above infinity
-      top = max(top, max(__float_as_uint(v[u][2 * j]) & 0x7FFFFFFFu, __float_as_uint(v[u][2 * j + 1]) & 0x7FFFFFFFu));
+      top = max_abs(max_abs(top, v[u][2 * j]), v[u][2 * j + 1]);
     }
   }
-  const RowScale s = row_scale(block_max(top, warp_max));
+  const RowScale s = row_scale(row_max(__float_as_uint(top), warp_max + threadIdx.y * (blockDim.x >> 5)));
+  if (!live) return;
   if (threadIdx.x == 0) p.scales[r] = s.scale;
   const bool zero = s.pre == 0.f;
   uint2* out = reinterpret_cast<uint2*>(p.codes + r * p.cols);
@@ -143,8 +163,8 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_rows_kernel(const QuantR
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float* x = &v[u][4 * h];
-      const uint32_t lo = __byte_perm(code_of(x[0], s), code_of(x[1], s), 0x0040);
-      const uint32_t hi = __byte_perm(code_of(x[2], s), code_of(x[3], s), 0x0040);
+      const uint32_t lo = __byte_perm(code_of<kAct>(x[0], s), code_of<kAct>(x[1], s), 0x0040);
+      const uint32_t hi = __byte_perm(code_of<kAct>(x[2], s), code_of<kAct>(x[3], s), 0x0040);
       q[h] = zero ? 0u : __byte_perm(lo, hi, 0x5410);
     }
     out[c] = make_uint2(q[0], q[1]);
@@ -155,6 +175,7 @@ template <int kAct>
 __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const QuantRowsParams p) {
   __shared__ uint32_t warp_max[2][kLongThreads / 32];
   let_dependents_start();
+  zero_words(p);
   int turn = 0;   // two sets of places: a warp may be one row ahead of another
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
     const int64_t src = source_row(p, r);
@@ -166,12 +187,12 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
         const float v = activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f);
         top = max(top, __float_as_uint(v) & 0x7FFFFFFFu);
       }
-    const RowScale s = row_scale(block_max(top, warp_max[turn]));
+    const RowScale s = row_scale(row_max(top, warp_max[turn]));
     if (threadIdx.x == 0) p.scales[r] = s.scale;
     const bool zero = s.pre == 0.f;
     for (int64_t c = threadIdx.x; c < p.cols; c += kLongThreads) {
       uint32_t q = 0;
-      if (!zero) q = code_of(activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f), s);
+      if (!zero) q = code_of<kAct>(activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f), s);
       p.codes[r * p.cols + c] = static_cast<int8_t>(q & 0xFFu);
     }
   }
@@ -181,14 +202,15 @@ template <int kAct>
 void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
   const int64_t vecs = p.cols / 8;
   const bool aligned = p.cols % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
-  if (aligned && vecs <= kMaxThreads * kMaxVecs && p.rows <= INT32_MAX) {
-    // as few vectors per thread as 512 threads allow: a row waits for its slowest load once
-    const int per = vecs <= kMaxThreads ? 1 : vecs <= 2 * kMaxThreads ? 2 : 4;
-    const int threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
-    const int grid = static_cast<int>(p.rows);
-    if (per == 1) quantize_rows_kernel<kAct, 1><<<grid, threads, 0, s>>>(p);
-    else if (per == 2) quantize_rows_kernel<kAct, 2><<<grid, threads, 0, s>>>(p);
-    else quantize_rows_kernel<kAct, 4><<<grid, threads, 0, s>>>(p);
+  if (aligned && vecs <= kMaxThreads * kVecs && p.rows <= INT32_MAX) {
+    // Two vectors per thread keep enough bytes in flight at 32 registers (32768 rows of 4096: 78 us, with one 113 us; behind
+    // SwiGLU 14336 wide 416 us, 5.6 TB/s); short rows share a block of 256 threads, since starting a block takes about 1 ns
+    // of the GPU's time (one row per block: 262144 rows of 1024 took 272 us).
+    const int threads = static_cast<int>(((vecs + 1) / 2 + 31) / 32 * 32);
+    const int rows_per_block = threads < 256 ? 256 / threads : 1;
+    const dim3 block(threads, rows_per_block);
+    const int64_t grid = (p.rows + rows_per_block - 1) / rows_per_block;
+    quantize_rows_kernel<kAct><<<static_cast<unsigned int>(grid), block, 0, s>>>(p);
     return;
   }
   const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
@@ -196,12 +218,8 @@ void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
 }
 
 }  // namespace
-}  // namespace fp8gmm
 
-extern "C" {
-
-int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) {
-  using namespace fp8gmm;
+int quantize_rows_launch(const fp8gmm_quantize_rows_args* a, void* zero, int zero_words, void* stream) {
   FP8GMM_CHECK_ARG(a != nullptr, "quantize_rows_int8: NULL arguments");
   FP8GMM_CHECK_ARG(a->rows >= 0 && a->cols >= 0 && a->in_rows >= 0, "quantize_rows_int8: negative size");
   FP8GMM_CHECK_ARG(a->activation == FP8GMM_ACT_NONE || a->activation == FP8GMM_ACT_GELU || a->activation == FP8GMM_ACT_SWIGLU,
@@ -223,6 +241,8 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) 
   p.cols = a->cols;
   p.codes = static_cast<int8_t*>(a->codes);
   p.scales = a->scales;
+  p.zero = static_cast<uint32_t*>(zero);
+  p.zero_words = zero_words;
   p.status = device_status_word();
   FP8GMM_CHECK_ARG(p.status != nullptr, "quantize_rows_int8: cannot resolve the device status word");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -232,6 +252,14 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) 
   FP8GMM_CHECK_CUDA(cudaGetLastError());
   count_launch();
   return FP8GMM_OK;
+}
+
+}  // namespace fp8gmm
+
+extern "C" {
+
+int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) {
+  return fp8gmm::quantize_rows_launch(a, nullptr, 0, stream);
 }
 
 }  // extern "C"
