@@ -36,7 +36,8 @@ constexpr int kWBytes = kChannels * kBlockK;
 
 struct Int8GemmParams {
   CUtensorMap map_w;                     // weights (G*N, K), box 128 rows x 128 bytes
-  CUtensorMap map_x;                     // codes (rows, K), box of half a tile's rows x 128 bytes
+  CUtensorMap map_x[3];                  // codes (rows, K), boxes of 32, 64 and 128 rows x 128 bytes (up to half of tile_rows): a tile
+                                         // with few rows loads no more than it needs
   uint16_t* c;
   const float* a_scales;
   const float* b_scales;
@@ -244,7 +245,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     prefetch_tensormap(&p.map_w);
-    prefetch_tensormap(&p.map_x);
+    for (int i = 0; i < 3; ++i)
+      if (64 << i <= p.tile_rows) prefetch_tensormap(&p.map_x[i]);
   }
   if (warp == 2) {
     tmem_alloc_pair(smem_u32(tmem_base_slot), kTmemCols);
@@ -269,18 +271,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
         const Tile t = decode_tile(p, row_start, tile_start, it.tile);
         const int width = (t.rows + 31) & ~31;                       // columns of this tile's MMAs, half of them from each CTA
         const int yw = t.group * p.n + t.n0 + rank * kChannels, yx = t.row0 + rank * (width / 2);
+        const int box = width <= 64 ? 0 : width <= 128 ? 1 : 2;       // box of 32 << box rows
+        const CUtensorMap* map_x = &p.map_x[box];
+        const int bytes = 2 * (kWBytes + (32 << box) * kBlockK);      // of both CTAs
         int kb = it.kb0;
         if (!waited) {
           // Weights do not depend on the kernel before this one (the quantisation of the rows): a ring full of them goes ahead.
           waited = true;
           const int first = min(it.kb1 - it.kb0, stages);
           for (int i = 0; i < first; ++i) {
-            if (leader) mbar_expect_tx(full_bar(i), 2 * stage_bytes);
+            if (leader) mbar_expect_tx(full_bar(i), bytes);
             tma_load_2d_pair(tiles_addr + i * stage_bytes, &p.map_w, full0_leader + 8u * i, (kb + i) * kBlockK, yw);
           }
           grid_dependency_wait();
           for (int i = 0; i < first; ++i)
-            tma_load_2d_pair(tiles_addr + i * stage_bytes + kWBytes, &p.map_x, full0_leader + 8u * i, (kb + i) * kBlockK, yx);
+            tma_load_2d_pair(tiles_addr + i * stage_bytes + kWBytes, map_x, full0_leader + 8u * i, (kb + i) * kBlockK, yx);
           kb += first;
           stage = first == stages ? 0 : first;
           phase = first == stages ? 1u : 0u;
@@ -289,9 +294,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
           ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x1, p.wait_ns);
           if (ok) {
             const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
-            if (leader) mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
+            if (leader) mbar_expect_tx(full_bar(stage), bytes);
             tma_load_2d_pair(sw, &p.map_w, bar, kb * kBlockK, yw);
-            tma_load_2d_pair(sw + kWBytes, &p.map_x, bar, kb * kBlockK, yx);
+            tma_load_2d_pair(sw + kWBytes, map_x, bar, kb * kBlockK, yx);
           }
           if (++stage == stages) {
             stage = 0;
@@ -583,8 +588,10 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
   p.tile_rows = tile_rows;
   rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, kChannels);
   if (rc != FP8GMM_OK) return rc;
-  rc = encode_rows(&p.map_x, a->a, a->rows, a->k, tile_rows / 2);
-  if (rc != FP8GMM_OK) return rc;
+  for (int i = 0; i < 3 && 64 << i <= tile_rows; ++i) {
+    rc = encode_rows(&p.map_x[i], a->a, a->rows, a->k, 32 << i);
+    if (rc != FP8GMM_OK) return rc;
+  }
   p.stage_bytes = kWBytes + tile_rows / 2 * kBlockK;
   p.stages = kRingBytes / p.stage_bytes < kMaxStages ? kRingBytes / p.stage_bytes : kMaxStages;
   p.tiles_n = (p.n + 2 * kChannels - 1) / (2 * kChannels);
