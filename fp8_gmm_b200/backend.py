@@ -727,8 +727,6 @@ def _int8_gemm_args(device, rows, k, b, group_sizes, b_scales, c, name):
         _fail(f"{name}: contraction dimensions differ")
     if not (b_scales.device == device and b_scales.dtype == torch.float32 and b_scales.shape == (G, n) and b_scales.is_contiguous()):
         _fail(f"{name}: the weights' scales must be (G, N) float32 on the device of the rows")
-    if len(group_sizes) != G:
-        _fail(f"{name}: one group size per expert is required")
     _no_grad_wanted(name, b_scales)
     if c is None:
         c = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
@@ -736,11 +734,15 @@ def _int8_gemm_args(device, rows, k, b, group_sizes, b_scales, c, name):
         _fail(f"{name}: bad output")
     args = Int8GemmArgs()
     keep = None
-    if torch.is_tensor(group_sizes) and group_sizes.is_cuda:
-        if not (group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.dim() == 1 and group_sizes.is_contiguous()):
+    if isinstance(group_sizes, torch.Tensor) and group_sizes.is_cuda:
+        if group_sizes.shape != (G,):
+            _fail(f"{name}: one group size per expert is required")
+        if not (group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.is_contiguous()):
             _fail(f"{name}: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of the rows")
         args.device_m_sizes = group_sizes.data_ptr()
     else:
+        if len(group_sizes) != G:
+            _fail(f"{name}: one group size per expert is required")
         args.m_sizes, keep = _i64_array(group_sizes)
     args.b, args.c, args.b_scales = b.data_ptr(), c.data_ptr(), b_scales.data_ptr()
     args.num_groups, args.rows, args.n, args.k = G, rows, n, k
@@ -813,32 +815,44 @@ def _dense(t):
     return True
 
 
-def _grad_descs(grads, outputs, name):
-    """Descriptor array (fp8gmm_grad_desc: in, out, numel, in_type | out_type << 32) and the common device."""
-    index = grads[0].get_device() if grads[0].is_cuda else None
-    if outputs is not None and len(outputs) != len(grads):
-        _fail(f"{name}: one output per gradient is required")
-    rows = []
+def _check_grads(grads, outputs, name):
+    """Raises for the first entry that the gradient kernels cannot take."""
+    index = grads[0].get_device()
     for i, g in enumerate(grads):
-        kind = _GRAD_TYPE.get(g.dtype)
-        if kind is None or not g.is_cuda or g.layout is not torch.strided:
+        if not g.is_cuda or g.layout is not torch.strided or g.dtype not in _GRAD_TYPE:
             _fail(f"{name}: gradient {i} must be a dense CUDA bfloat16, float16 or float32 tensor")
         if g.get_device() != index:
             _fail(f"{name}: gradient {i} is on another device than gradient 0")
-        plain = g.is_contiguous()
-        if not plain and not _dense(g):
+        if not _dense(g):
             _fail(f"{name}: gradient {i} has gaps or shares elements with itself")
-        ptr = out_ptr = g.data_ptr()
-        out_kind = kind
         if outputs is not None:
             o = outputs[i]
-            out_kind = _GRAD_TYPE.get(o.dtype)
-            if out_kind is None or not o.is_cuda or o.get_device() != index:
+            if not o.is_cuda or o.get_device() != index or o.dtype not in _GRAD_TYPE:
                 _fail(f"{name}: output {i} must be a bfloat16, float16 or float32 tensor on the device of the gradients")
-            if o.shape != g.shape or not (plain and o.is_contiguous() or o.stride() == g.stride()):
+            if o.shape != g.shape or not (g.is_contiguous() and o.is_contiguous() or o.stride() == g.stride()):
                 _fail(f"{name}: output {i} does not have the layout of its gradient")
-            out_ptr = o.data_ptr()
-        rows += (ptr, out_ptr, g.numel(), kind | out_kind << 32)
+
+
+def _plain(tensors, index):
+    """Whether all are contiguous tensors of the kernels' types on the CUDA device ``index``."""
+    return (index >= 0 and all([t.is_contiguous() for t in tensors]) and all([t.dtype in _GRAD_TYPE for t in tensors])
+            and all([t.get_device() == index for t in tensors]))
+
+
+def _grad_descs(grads, outputs, name):
+    """Descriptor array (fp8gmm_grad_desc: in, out, numel, in_type | out_type << 32) and the common device."""
+    if outputs is not None and len(outputs) != len(grads):
+        _fail(f"{name}: one output per gradient is required")
+    dense = all([g.layout is torch.strided for g in grads])
+    index = grads[0].get_device()
+    if not (dense and _plain(grads, index)
+            and (outputs is None or _plain(outputs, index) and [g.shape for g in grads] == [o.shape for o in outputs])):
+        _check_grads(grads, outputs, name)
+    if outputs is None:
+        rows = [v for g in grads for v in (g.data_ptr(), g.data_ptr(), g.numel(), _GRAD_TYPE[g.dtype] * 0x100000001)]
+    else:
+        rows = [v for g, o in zip(grads, outputs)
+                for v in (g.data_ptr(), o.data_ptr(), g.numel(), _GRAD_TYPE[g.dtype] | _GRAD_TYPE[o.dtype] << 32)]
     return (ctypes.c_int64 * len(rows))(*rows), grads[0].device
 
 

@@ -21,8 +21,8 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kLongThreads = 256;
-constexpr int kMaxThreads = 1024;
-constexpr int kVecs = 2;                 // 8-element vectors a thread holds: rows of up to 1024 * 2 * 8 = 16384 elements
+constexpr int kMaxThreads = 512;
+constexpr int kMaxVecs = 4;              // 8-element vectors a thread holds: rows of up to 512 * 4 * 8 = 16384 elements
 constexpr int kStatusBadIndex = 0x200;   // as in routing.cu: an index that names no row
 
 struct QuantRowsParams {
@@ -118,8 +118,8 @@ __device__ __forceinline__ int64_t source_row(const QuantRowsParams& p, int64_t 
   return -1;
 }
 
-template <int kAct>
-__global__ void __launch_bounds__(kMaxThreads, 2) quantize_rows_kernel(const QuantRowsParams p) {
+template <int kAct, int kVecs>
+__global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_ACT_SWIGLU ? 2 : 3) quantize_rows_kernel(const QuantRowsParams p) {
   __shared__ uint32_t warp_max[kMaxThreads / 32];
   let_dependents_start();
   zero_words(p);
@@ -202,15 +202,18 @@ template <int kAct>
 void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
   const int64_t vecs = p.cols / 8;
   const bool aligned = p.cols % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
-  if (aligned && vecs <= kMaxThreads * kVecs && p.rows <= INT32_MAX) {
-    // Two vectors per thread keep enough bytes in flight at 32 registers (32768 rows of 4096: 78 us, with one 113 us; behind
-    // SwiGLU 14336 wide 416 us, 5.6 TB/s); short rows share a block of 256 threads, since starting a block takes about 1 ns
-    // of the GPU's time (one row per block: 262144 rows of 1024 took 272 us).
-    const int threads = static_cast<int>(((vecs + 1) / 2 + 31) / 32 * 32);
+  if (aligned && vecs <= kMaxThreads * kMaxVecs && p.rows <= INT32_MAX) {
+    // Four vectors per thread keep more bytes in flight (measured against two: 32768 rows of 4096 70 / 81 us, behind SwiGLU
+    // 14336 wide 392 / 434 us = 6.0 TB/s); two answer sooner where all rows run at once, and fill a warp with a short row
+    // (100000 rows of 272: 29 / 37 us).  Short rows share a block, since starting a block takes about 1 ns of the GPU's
+    // time (one row per block: 262144 rows of 1024 took 272 us, now 129).
+    const int per = vecs <= 64 || (vecs <= 2 * kMaxThreads && p.rows <= 4 * sm_count()) ? 2 : 4;
+    const int threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
     const int rows_per_block = threads < 256 ? 256 / threads : 1;
     const dim3 block(threads, rows_per_block);
-    const int64_t grid = (p.rows + rows_per_block - 1) / rows_per_block;
-    quantize_rows_kernel<kAct><<<static_cast<unsigned int>(grid), block, 0, s>>>(p);
+    const unsigned int grid = static_cast<unsigned int>((p.rows + rows_per_block - 1) / rows_per_block);
+    if (per == 2) quantize_rows_kernel<kAct, 2><<<grid, block, 0, s>>>(p);
+    else quantize_rows_kernel<kAct, 4><<<grid, block, 0, s>>>(p);
     return;
   }
   const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
