@@ -87,7 +87,6 @@ class Int8GemmArgs(ctypes.Structure):
         ("a", c_vp), ("b", c_vp), ("c", c_vp), ("a_scales", c_fp), ("b_scales", c_fp),
         ("m_sizes", ctypes.POINTER(c_i64)), ("device_m_sizes", c_vp),
         ("num_groups", ctypes.c_int), ("rows", c_i64), ("n", c_i64), ("k", c_i64),
-        ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -129,9 +128,8 @@ SYMBOLS = {
     "fp8gmm_moe_rowdot": (ctypes.c_int, [c_vp, c_vp, c_vp, ctypes.c_int, c_i64, c_i64, c_vp, c_vp]),
     "fp8gmm_quantize_rows_int8": (ctypes.c_int, [ctypes.POINTER(QuantizeRowsArgs), c_vp]),
     "fp8gmm_int8_grouped_gemm": (ctypes.c_int, [ctypes.POINTER(Int8GemmArgs), c_vp]),
-    "fp8gmm_int8_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Int8GemmArgs)]),
     "fp8gmm_int8_linear": (ctypes.c_int, [ctypes.POINTER(QuantizeRowsArgs), ctypes.POINTER(Int8GemmArgs), c_vp]),
-    "fp8gmm_set_int8_variant": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
+    "fp8gmm_set_int8_variant": (ctypes.c_int, [ctypes.c_int]),
     "fp8gmm_sum_squares_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int]),
     "fp8gmm_multi_sum_squares": (ctypes.c_int, [c_vp, ctypes.c_int, c_vp, ctypes.c_size_t, c_vp, c_fp, c_vp]),
     "fp8gmm_multi_clip": (ctypes.c_int, [c_vp, ctypes.c_int, c_vp, ctypes.c_float, c_fp, c_vp]),

@@ -75,10 +75,10 @@ def set_gemm_variant(ctas=0, tail_split=True, tma_epilogue=True):
     check(lib.fp8gmm_set_gemm_variant(int(ctas), int(bool(tail_split)), int(bool(tma_epilogue))), "set_gemm_variant")
 
 
-def set_int8_variant(tile_rows=0, split=True):
-    """Force the rows of the int8 product's tiles (64, 128 or 256; 0 = automatic), and forbid splitting the tiles of a
-    partial wave; see fp8gmm_set_int8_variant.  For tests and experiments: results are bit-identical."""
-    check(lib.fp8gmm_set_int8_variant(int(tile_rows), int(split)), "set_int8_variant")
+def set_int8_variant(tile_rows=0):
+    """Force the rows of the int8 product's tiles (128 or 256; 0 = automatic); see fp8gmm_set_int8_variant.  For tests and
+    experiments: results are bit-identical."""
+    check(lib.fp8gmm_set_int8_variant(int(tile_rows)), "set_int8_variant")
 
 
 def set_wait_limits(gemm_wait_s=0.0, peer_wait_s=0.0):
@@ -765,10 +765,6 @@ def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
     args, c, keep = _int8_gemm_args(a.device, rows, k, b, group_sizes, b_scales, c, "int8_gmm")
     args.a, args.a_scales = a.data_ptr(), a_scales.data_ptr()
     with _on(a.device):
-        # taken per call, not kept: graphs captured one after the other would share a buffer that is kept
-        args.workspace_bytes = nbytes = lib.fp8gmm_int8_workspace_bytes(ctypes.byref(args))
-        ws = torch.empty(nbytes, dtype=torch.int8, device=a.device) if nbytes else None
-        args.workspace = _ptr(ws)
         check(lib.fp8gmm_int8_grouped_gemm(ctypes.byref(args), _stream()), "int8_gmm")
     del keep
     return c
@@ -785,13 +781,11 @@ def int8_linear(x, weight, group_sizes, weight_scales, indices=None, top_k=1, ac
     q, (rows,) = _quantize_args(x, indices, top_k, activation)
     k = q.cols
     g, c, keep = _int8_gemm_args(x.device, rows, k, weight, group_sizes, weight_scales, c, "int8_linear")
+    # codes, then scales (K is a multiple of 16), taken per call: graphs captured one after the other would share a buffer that is kept
+    scratch = torch.empty(rows * (k + 4), dtype=torch.int8, device=x.device)
+    q.codes = g.a = scratch.data_ptr()
+    q.scales = g.a_scales = scratch.data_ptr() + rows * k
     with _on(x.device):
-        # one buffer per call: the product's workspace, the codes, their scales (K is a multiple of 16)
-        g.workspace_bytes = nbytes = lib.fp8gmm_int8_workspace_bytes(ctypes.byref(g)) + 15 & -16
-        scratch = torch.empty(nbytes + rows * (k + 4), dtype=torch.int8, device=x.device)
-        g.workspace = scratch.data_ptr()
-        q.codes = g.a = g.workspace + nbytes if rows else None
-        q.scales = g.a_scales = g.a + rows * k if rows else None
         check(lib.fp8gmm_int8_linear(ctypes.byref(q), ctypes.byref(g), _stream()), "int8_linear")
     del keep
     return c
@@ -833,26 +827,26 @@ def _check_grads(grads, outputs, name):
                 _fail(f"{name}: output {i} does not have the layout of its gradient")
 
 
-def _plain(tensors, index):
-    """Whether all are contiguous tensors of the kernels' types on the CUDA device ``index``."""
-    return (index >= 0 and all([t.is_contiguous() for t in tensors]) and all([t.dtype in _GRAD_TYPE for t in tensors])
-            and all([t.get_device() == index for t in tensors]))
+def _kinds(tensors, index):
+    """Type codes of the tensors if all are contiguous ones of the kernels' types on the CUDA device ``index``, else None."""
+    kinds = [_GRAD_TYPE.get(t.dtype) for t in tensors]
+    if index < 0 or None in kinds or not all([t.get_device() == index and t.is_contiguous() for t in tensors]):
+        return None
+    return kinds
 
 
 def _grad_descs(grads, outputs, name):
     """Descriptor array (fp8gmm_grad_desc: in, out, numel, in_type | out_type << 32) and the common device."""
     if outputs is not None and len(outputs) != len(grads):
         _fail(f"{name}: one output per gradient is required")
-    dense = all([g.layout is torch.strided for g in grads])
     index = grads[0].get_device()
-    if not (dense and _plain(grads, index)
-            and (outputs is None or _plain(outputs, index) and [g.shape for g in grads] == [o.shape for o in outputs])):
-        _check_grads(grads, outputs, name)
-    if outputs is None:
-        rows = [v for g in grads for v in (g.data_ptr(), g.data_ptr(), g.numel(), _GRAD_TYPE[g.dtype] * 0x100000001)]
-    else:
-        rows = [v for g, o in zip(grads, outputs)
-                for v in (g.data_ptr(), o.data_ptr(), g.numel(), _GRAD_TYPE[g.dtype] | _GRAD_TYPE[o.dtype] << 32)]
+    kinds = _kinds(grads, index)
+    out_kinds = kinds if outputs is None else _kinds(outputs, index)
+    if kinds is None or out_kinds is None or outputs is not None and any([g.shape != o.shape for g, o in zip(grads, outputs)]):
+        _check_grads(grads, outputs, name)   # the slow way round: permuted dense tensors, or what is wrong
+        kinds = [_GRAD_TYPE[g.dtype] for g in grads]
+        out_kinds = kinds if outputs is None else [_GRAD_TYPE[o.dtype] for o in outputs]
+    rows = [v for g, o, k, ok in zip(grads, outputs or grads, kinds, out_kinds) for v in (g.data_ptr(), o.data_ptr(), g.numel(), k | ok << 32)]
     return (ctypes.c_int64 * len(rows))(*rows), grads[0].device
 
 

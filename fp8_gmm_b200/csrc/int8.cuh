@@ -5,12 +5,8 @@
 
 namespace fp8gmm {
 
-// fp8gmm_quantize_rows_int8, which also zeroes `zero_words` 32-bit words at `zero` (unless NULL).
-int quantize_rows_launch(const fp8gmm_quantize_rows_args* a, void* zero, int zero_words, void* stream);
-
 // The product of rows that `fp8gmm_quantize_rows_int8` has just been enqueued for on the same stream: its CTAs may start, and
-// load weights, before the codes are there.  after_quantize: that is so, and
-// the quantisation has zeroed the workspace's counters.
+// load weights, before the codes are there (after_quantize).
 int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_quantize);
 
 }  // namespace fp8gmm

@@ -9,13 +9,9 @@
 // The operands are swapped against gemm_sm100.cu: output channels are the M dimension of the MMA (TMEM lanes), rows the N
 // dimension (TMEM columns).  A group of any number of rows then costs an MMA only as wide as its rows, and a warp's 32 lanes
 // hold 32 neighbouring channels of one output row.
-//   * Persistent CTA pairs (cta_group::2): a tile is 256 channels x up to 64, 128 or 256 rows; each CTA loads its 128 channels
-//     of weights and half of the tile's rows; ring of 6 (256 rows) to 9 (64 rows) stages of 128 contraction bytes, accumulators
-//     double-buffered in TMEM, results transposed through shared memory and written as 256-byte runs.
-//   * The tiles that fill whole waves of the grid go to the pairs one after another; with few rows those of the last, partial wave
-//     are cut along the contraction so that every pair gets an equal share.  A pair that did a part of a tile leaves its sums in a workspace
-//     and counts itself in; the last one to come adds all parts up (integers: any order gives the same bits) and finishes the
-//     tile.  Nobody waits for anybody.
+//   * Persistent CTA pairs (cta_group::2): a tile is 256 channels x up to 128 or 256 rows; each CTA loads its 128 channels of
+//     weights and half of the tile's rows, 128 contraction bytes per stage, into a ring of 8 or 6 stages.
+//   * Accumulators are double-buffered in TMEM; results are transposed through shared memory and written as 256-byte runs.
 // Group sizes come from the host (parameter block) or are read on the device; either way every CTA builds the prefix sums of
 // rows and tiles in shared memory.  Waits on mbarriers are bounded as in gemm_sm100.cu.
 #include <atomic>
@@ -36,18 +32,17 @@ constexpr int kWBytes = kChannels * kBlockK;
 
 struct Int8GemmParams {
   CUtensorMap map_w;                     // weights (G*N, K), box 128 rows x 128 bytes
-  CUtensorMap map_x[3];                  // codes (rows, K), boxes of 32, 64 and 128 rows x 128 bytes (up to half of tile_rows): a tile
-                                         // with few rows loads no more than it needs
+  CUtensorMap map_x[4];                  // codes (rows, K), boxes of 16, 32, 64 and 128 rows x 128 bytes (up to half of tile_rows): a
+                                         // tile with few rows loads no more than it needs
   uint16_t* c;
   const float* a_scales;
   const float* b_scales;
   const int64_t* device_sizes;           // group sizes on the device, or NULL: row_start holds their prefix sums
-  unsigned int* counters;                // workspace: parts that have come per split tile and CTA of the pair, zeroed
-  int* parts;                            // workspace: sums of parts, [pair][CTA][first, last][row][channel]; NULL = no splitting
   int* status;
   unsigned long long wait_ns;
   int num_groups, rows, n, k;
   int tile_rows, tiles_n, super_tiles;
+  int x_maps;                            // entries of map_x that a tile can need
   int stages, stage_bytes;
   int row_start[kMaxGroups + 1];
 };
@@ -65,13 +60,6 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_w, u
 // [24,29) M >> 4; both operands K-major.
 __device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
 }
 
 __device__ __forceinline__ uint16_t result_bf16(uint32_t acc, float scale) {
@@ -147,58 +135,8 @@ __device__ __forceinline__ Tile decode_tile(const Int8GemmParams& p, const int* 
   return t;
 }
 
-// The work of one pair: whole tiles of the full waves, then its share of the last wave.
-struct Item {
-  int tile, kb0, kb1;
-  int rest;   // number of the tile in the last wave if that is split, else -1
-};
-struct Schedule {
-  int workers, worker, num_kb, full, rest, sharers, units;   // units: K blocks of the last wave
-  int i, u, u_end;
-
-  __device__ __forceinline__ Schedule(int worker_, int workers_, int total_tiles, int num_kb_, bool may_split)
-      : workers(workers_), worker(worker_), num_kb(num_kb_), full(total_tiles / workers_), rest(total_tiles - full * workers_), sharers(0),
-        units(rest * num_kb_), i(0), u(0), u_end(0) {
-    const int most = min(workers, units / kMinShare);
-    if (may_split && most > 0 && num_kb - (units + most - 1) / most >= kMinGain) {
-      sharers = most;
-      if (worker < sharers) {
-        u = begin_of(worker);
-        u_end = begin_of(worker + 1);
-      }
-    }
-  }
-  // The parts' way through L2 takes about 5 us, as long as 14 K blocks of weights: splitting has to save more.  (Measured with one
-  // row: 8 tiles of 56 K blocks 23.0 -> 13.2 us, 32 tiles of 112 41.4 -> 30.5, 32 tiles of 32 16.6 -> 16.9; with 54 tiles of 32 in
-  // the last wave, 9 K blocks to save, 29.5 -> 31.9.)
-  static constexpr int kMinGain = 16;
-  static constexpr int kMinShare = 8;
-  __device__ __forceinline__ int begin_of(int w) const { return static_cast<int>(static_cast<long long>(units) * w / sharers); }
-  // The pair whose share holds unit `at`.
-  __device__ __forceinline__ int sharer_of(int at) const {
-    return static_cast<int>((static_cast<long long>(at + 1) * sharers - 1) / units);
-  }
-  __device__ __forceinline__ bool next(Item& it) {
-    it.kb0 = 0;
-    it.kb1 = num_kb;
-    it.rest = -1;
-    if (i < full || (i == full && sharers == 0 && worker < rest)) {
-      it.tile = worker + i * workers;
-      ++i;
-      return true;
-    }
-    if (u >= u_end) return false;
-    it.rest = u / num_kb;
-    it.tile = full * workers + it.rest;
-    it.kb0 = u - it.rest * num_kb;
-    it.kb1 = min(num_kb, it.kb0 + u_end - u);
-    u += it.kb1 - it.kb0;
-    return true;
-  }
-};
-
-constexpr int kMinRows = 64, kMaxRows = 256;  // rows of the smallest and the largest tile
-constexpr int kMaxStages = 9;
+constexpr int kMaxRows = 256;                 // rows of the larger tile
+constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 6 * 32 * 1024;
 constexpr int kTmemCols = 512;
 constexpr int kBoxBytes = 32 * kChannels * 2; // 32 rows x 128 channels of bf16
@@ -206,6 +144,16 @@ constexpr int kStagingBytes = 2 * kBoxBytes;
 constexpr int kScaleBytes = 2 * kMaxRows * 4;
 constexpr int kTableBytes = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
 constexpr int kSmemBytes = kRingBytes + kStagingBytes + kScaleBytes + kTableBytes + 1024 + 256;
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Columns of a tile's MMAs; half of its rows come from each CTA.
+__device__ __forceinline__ int mma_width(int rows) { return (rows + 31) & ~31; }
 
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -225,7 +173,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
   auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 2 + a); };
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
-  volatile int* finish_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -245,8 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     prefetch_tensormap(&p.map_w);
-    for (int i = 0; i < 3; ++i)
-      if (64 << i <= p.tile_rows) prefetch_tensormap(&p.map_x[i]);
+    for (int i = 0; i < p.x_maps; ++i) prefetch_tensormap(&p.map_x[i]);
   }
   if (warp == 2) {
     tmem_alloc_pair(smem_u32(tmem_base_slot), kTmemCols);
@@ -257,84 +203,87 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
-  Schedule work(blockIdx.x >> 1, gridDim.x >> 1, tile_start[p.num_groups], (p.k + kBlockK - 1) / kBlockK, p.parts != nullptr);
-  Item it;
+  const int worker = blockIdx.x >> 1, num_workers = gridDim.x >> 1;
+  const int total_tiles = tile_start[p.num_groups];
+  const int num_kb = (p.k + kBlockK - 1) / kBlockK;
 
   if (warp == 0) {
     // ===================== TMA producer: both CTAs credit the leader's barriers =====================
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true, waited = false;
-      const uint32_t full0_leader = map_to_cta(full_bar(0), 0);
-      while (ok && work.next(it)) {
-        const Tile t = decode_tile(p, row_start, tile_start, it.tile);
-        const int width = (t.rows + 31) & ~31;                       // columns of this tile's MMAs, half of them from each CTA
-        const int yw = t.group * p.n + t.n0 + rank * kChannels, yx = t.row0 + rank * (width / 2);
-        const int box = width <= 64 ? 0 : width <= 128 ? 1 : 2;       // box of 32 << box rows
-        const CUtensorMap* map_x = &p.map_x[box];
-        const int bytes = 2 * (kWBytes + (32 << box) * kBlockK);      // of both CTAs
-        int kb = it.kb0;
-        if (!waited) {
-          // Weights do not depend on the kernel before this one (the quantisation of the rows): a ring full of them goes ahead.
-          waited = true;
-          const int first = min(it.kb1 - it.kb0, stages);
-          for (int i = 0; i < first; ++i) {
-            if (leader) mbar_expect_tx(full_bar(i), bytes);
-            tma_load_2d_pair(tiles_addr + i * stage_bytes, &p.map_w, full0_leader + 8u * i, (kb + i) * kBlockK, yw);
-          }
-          grid_dependency_wait();
-          for (int i = 0; i < first; ++i)
-            tma_load_2d_pair(tiles_addr + i * stage_bytes + kWBytes, map_x, full0_leader + 8u * i, (kb + i) * kBlockK, yx);
-          kb += first;
-          stage = first == stages ? 0 : first;
-          phase = first == stages ? 1u : 0u;
+    // The whole warp walks the loop and one elected lane issues: code under a test of the lane number cannot keep its operands in
+    // uniform registers, and the MMA warp's loop took 300 ns a K block that way instead of 200 (one tile of 256 x 1).
+    const bool issue = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t full0_leader = map_to_cta(full_bar(0), 0);
+    for (int tile = worker; tile < total_tiles && ok; tile += num_workers) {
+      const Tile t = decode_tile(p, row_start, tile_start, tile);
+      const int width = mma_width(t.rows);
+      const int yw = t.group * p.n + t.n0 + rank * kChannels, yx = t.row0 + rank * (width / 2);
+      const int box = width <= 32 ? 0 : width <= 64 ? 1 : width <= 128 ? 2 : 3;   // box of 16 << box rows: one CTA's half
+      const CUtensorMap* map_x = &p.map_x[box];
+      const int bytes = 2 * (kWBytes + (16 << box) * kBlockK);                    // of both CTAs
+      int kb = 0;
+      if (tile == worker) {
+        // Weights do not depend on the kernel before this one (the quantisation of the rows): a ring full of them goes ahead.
+        const int first = min(num_kb, stages);
+        for (int i = 0; i < first; ++i) {
+          if (leader && issue) mbar_expect_tx(full_bar(i), bytes);
+          if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes, &p.map_w, full0_leader + 8u * i, i * kBlockK, yw);
         }
-        for (; kb < it.kb1 && ok; ++kb) {
-          ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x1, p.wait_ns);
-          if (ok) {
-            const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
-            if (leader) mbar_expect_tx(full_bar(stage), bytes);
-            tma_load_2d_pair(sw, &p.map_w, bar, kb * kBlockK, yw);
-            tma_load_2d_pair(sw + kWBytes, map_x, bar, kb * kBlockK, yx);
-          }
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        grid_dependency_wait();
+        for (int i = 0; i < first; ++i)
+          if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes + kWBytes, map_x, full0_leader + 8u * i, i * kBlockK, yx);
+        kb = first;
+        stage = first == stages ? 0 : first;
+        phase = first == stages ? 1u : 0u;
+      }
+      for (; kb < num_kb && ok; ++kb) {
+        ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x1, p.wait_ns);
+        if (ok) {
+          const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
+          if (leader && issue) mbar_expect_tx(full_bar(stage), bytes);
+          if (issue) tma_load_2d_pair(sw, &p.map_w, bar, kb * kBlockK, yw);
+          if (issue) tma_load_2d_pair(sw + kWBytes, map_x, bar, kb * kBlockK, yx);
+        }
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ===================== MMA issuer: one thread of the leader =====================
-    if (leader && lane == 0) {
+    // ===================== MMA issuer: one lane of the leader =====================
+    if (leader) {
+      const bool issue = elect_one();
       const uint64_t desc_w0 = make_smem_desc(tiles_addr), desc_x0 = make_smem_desc(tiles_addr + kWBytes);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      while (ok && work.next(it)) {
-        const Tile t = decode_tile(p, row_start, tile_start, it.tile);
-        const uint32_t idesc = idesc_i8(2 * kChannels, (t.rows + 31) & ~31);
+      for (int tile = worker; tile < total_tiles; tile += num_workers) {
+        const Tile t = decode_tile(p, row_start, tile_start, tile);
+        const uint32_t idesc = idesc_i8(2 * kChannels, mma_width(t.rows));
         ok = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.status, 0x2, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kMaxRows);
-        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+        for (int kb = 0; kb < num_kb; ++kb) {
           ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, 0x4, p.wait_ns);
           if (!ok) break;
           const uint64_t dw = desc_w0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
           const uint64_t dx = desc_x0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k) umma_i8_pair(tmem_d, dw + 2 * k, dx + 2 * k, idesc, (kb != it.kb0 || k != 0) ? 1u : 0u);
-          umma_commit_pair(empty_bar(stage));
+          for (int k = 0; k < kBlockK / 32; ++k)
+            if (issue) umma_i8_pair(tmem_d, dw + 2 * k, dx + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          if (issue) umma_commit_pair(empty_bar(stage));
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        umma_commit_pair(tfull_bar(acc));
+        if (issue) umma_commit_pair(tfull_bar(acc));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }
@@ -348,8 +297,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     uint32_t acc_phase = 0;
     bool ok = true;
     grid_dependency_wait();
-    while (work.next(it)) {
-      const Tile t = decode_tile(p, row_start, tile_start, it.tile);
+    for (int tile = worker; tile < total_tiles; tile += num_workers) {
+      const Tile t = decode_tile(p, row_start, tile_start, tile);
       const int n0 = t.n0 + rank * kChannels;
       const int channel = n0 + quad * 32 + lane;
       const float sb = channel < p.n ? p.b_scales[static_cast<int64_t>(t.group) * p.n + channel] : 0.f;
@@ -361,95 +310,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
       tc_fence_after();
       const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * kMaxRows) + (static_cast<uint32_t>(quad * 32) << 16);
 
-      bool finish = true;
-      int first_sharer = 0, last_sharer = -1, tile_begin = 0;
-      const int64_t part_stride = static_cast<int64_t>(p.tile_rows) * kChannels;
-      if (it.rest >= 0 && it.kb1 - it.kb0 < work.num_kb) {
-        // Part of a tile: its sums go to the workspace, in the place of this pair's first or last tile.
-        tile_begin = it.rest * work.num_kb;
-        first_sharer = work.sharer_of(tile_begin);
-        last_sharer = work.sharer_of(tile_begin + work.num_kb - 1);
-        const int place = tile_begin + it.kb0 == work.begin_of(work.worker) ? 0 : 1;
-        const int rows8 = (t.rows + 7) & ~7;
+      for (int c0 = 0; c0 < t.rows; c0 += 32) {
+        uint16_t* box = reinterpret_cast<uint16_t*>(staging + ((c0 >> 5) & 1) * kBoxBytes);
         if (ok) {
-          int* out = p.parts + ((static_cast<int64_t>(work.worker) * 2 + rank) * 2 + place) * part_stride + quad * 32 + lane;
-          for (int c0 = 0; c0 < rows8; c0 += 8) {
-            uint32_t r[8];
-            tmem_ld8(taddr + c0, r);
-            tc_wait_ld();
+          uint32_t r[32];
+          tmem_ld32(taddr + c0, r);
+          tc_wait_ld();
+          uint16_t* mine = box + quad * 32 + lane;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) __stcg(out + (c0 + j) * kChannels, static_cast<int>(r[j]));
+          for (int j = 0; j < 32; j += 4) {
+            const float4 sa = *reinterpret_cast<const float4*>(scales + c0 + j);
+            mine[(j + 0) * kChannels] = result_bf16(r[j + 0], __fmul_rn(sa.x, sb));
+            mine[(j + 1) * kChannels] = result_bf16(r[j + 1], __fmul_rn(sa.y, sb));
+            mine[(j + 2) * kChannels] = result_bf16(r[j + 2], __fmul_rn(sa.z, sb));
+            mine[(j + 3) * kChannels] = result_bf16(r[j + 3], __fmul_rn(sa.w, sb));
           }
         }
         epilogue_barrier();
-        if (thread == 0) {
-          // behind the barrier this thread has seen the others' stores: its release covers them, its acquire what they read next
-          __threadfence();
-          const unsigned int before = atomicAdd(p.counters + it.rest * 2 + rank, 1u);
-          __threadfence();
-          *finish_flag = before == static_cast<unsigned int>(last_sharer - first_sharer);
-        }
-        epilogue_barrier();
-        finish = *finish_flag != 0;
-      }
-      if (finish) {
-        for (int c0 = 0; c0 < t.rows; c0 += 32) {
-          uint16_t* box = reinterpret_cast<uint16_t*>(staging + ((c0 >> 5) & 1) * kBoxBytes);
-          if (ok) {
-            uint32_t r[32];
-            tmem_ld32(taddr + c0, r);
-            tc_wait_ld();
-            if (last_sharer >= first_sharer) {
-              // the others' parts, eight rows of up to four of them in flight
+        // 16 threads write the 256 bytes of a row; the box is free again after the next barrier
+        const int chunk = thread & 15;
+        if (ok && n0 + chunk * 8 < p.n) {
 #pragma unroll
-              for (int j0 = 0; j0 < 32; j0 += 8) {
-                if (c0 + j0 >= t.rows) break;
-                for (int w0 = first_sharer; w0 <= last_sharer; w0 += 4) {
-                  int other[4][8];
-#pragma unroll
-                  for (int v = 0; v < 4; ++v) {
-                    const int w = w0 + v;
-                    const bool there = w <= last_sharer && w != work.worker;
-                    const int place = there && work.begin_of(w) >= tile_begin ? 0 : 1;
-                    const int* in = p.parts + ((static_cast<int64_t>(w) * 2 + rank) * 2 + place) * part_stride + quad * 32 + lane;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) other[v][j] = there ? __ldcg(in + (c0 + j0 + j) * kChannels) : 0;
-                  }
-#pragma unroll
-                  for (int v = 0; v < 4; ++v)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) r[j0 + j] += static_cast<uint32_t>(other[v][j]);
-                }
-              }
-            }
-            uint16_t* mine = reinterpret_cast<uint16_t*>(box) + quad * 32 + lane;
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 sa = *reinterpret_cast<const float4*>(scales + c0 + j);
-              mine[(j + 0) * kChannels] = result_bf16(r[j + 0], __fmul_rn(sa.x, sb));
-              mine[(j + 1) * kChannels] = result_bf16(r[j + 1], __fmul_rn(sa.y, sb));
-              mine[(j + 2) * kChannels] = result_bf16(r[j + 2], __fmul_rn(sa.z, sb));
-              mine[(j + 3) * kChannels] = result_bf16(r[j + 3], __fmul_rn(sa.w, sb));
-            }
-          }
-          epilogue_barrier();
-          // 16 threads write the 256 bytes of a row; the box is free again after the next barrier
-          const int chunk = thread & 15;
-          if (ok && n0 + chunk * 8 < p.n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = i * 8 + (thread >> 4);
-              if (c0 + row < t.rows)
-                *reinterpret_cast<uint4*>(p.c + static_cast<int64_t>(t.row0 + c0 + row) * p.n + n0 + chunk * 8) =
-                    *reinterpret_cast<const uint4*>(box + row * kChannels + chunk * 8);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (thread >> 4);
+            if (c0 + row < t.rows)
+              *reinterpret_cast<uint4*>(p.c + static_cast<int64_t>(t.row0 + c0 + row) * p.n + n0 + chunk * 8) =
+                  *reinterpret_cast<const uint4*>(box + row * kChannels + chunk * 8);
           }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(map_to_cta(tempty_bar(acc), 0));
-      epilogue_barrier();     // the last box and the flag are read before the next tile writes them
+      epilogue_barrier();     // the last box is read before the next tile writes into it
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
@@ -494,9 +387,6 @@ int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, 
 
 // Process-wide override for tests (fp8gmm_set_int8_variant): 0 = chosen per call.
 int g_tile_rows = 0;
-int g_split = 1;
-
-constexpr int kCounterBytes = 1024;   // two counters for each tile of a partial wave (fewer tiles than pairs)
 
 // Once per device: the attribute stays.
 int allow_shared_memory() {
@@ -512,30 +402,19 @@ int allow_shared_memory() {
 
 int pairs() { return sm_count() / 2; }
 
-// Rows of a tile.  Few rows per group: smaller tiles leave more stages for weights in flight and compute less on empty columns
-// (20 GB/s of weights per SM more with 64 than with 256); many: larger ones read the weights less often.  Measured, product
-// and quantisation, us (64 / 128 / 256 rows): eight experts of 4096 x 4096 with 8 rows each 29.5 / 29.8 / 29.8, with 32 rows
-// 34.2 / 32.0 / 32.6, with 128 rows 62.6 / 47.9 / 40.7; 64 experts of 1424 x 2048 with 8 rows 38.6 / 38.7 / 40.0, with 64 rows
-// 64.1 / 53.6 / 54.7, with 256 rows 171 / 117 / 97.  A grid that would not be filled takes smaller tiles: one expert of
-// 1024 x 4096 with 1024 rows 21.0 / 21.6 / 22.7; 4096 x 14336 with 300 rows 78 (second wave) / 45.9 / 47.3.
+// Rows of a tile: 256, which reads the weights least often, or 128 for groups of up to 64 rows (two more stages in flight) and where
+// smaller tiles still fit one wave of the grid.  It goes by the mean rows of a group that can have any, so that sizes on the
+// host and on the device take the same tile.  Measured, product and quantisation, us (128 / 256 rows): eight experts of 4096 x
+// 4096 with 8 rows each 25.8 / 26.6, with 32 rows 29.5 / 30.0, with 64 rows 32.0 / 31.7, with 256 rows 49.4 / 47.0, with 1024 rows 138 / 117;
+// one expert of 1024 x 4096 with 1024 rows 15.4 / 20.3, of 4096 x 14336 with 300 rows 33.8 / 45.3.  (Tiles of 64 rows: 25.7 and
+// 14.9 at best.  Splitting the contraction of the tiles of a partial wave between pairs, with sums handed on through L2, cost about
+// 8 us a tile and paid only below 16 tiles: dropped.)
 int choose_tile_rows(const fp8gmm_int8_gemm_args* a) {
   if (g_tile_rows != 0) return g_tile_rows;
   const int64_t tiles_n = (a->n + 2 * kChannels - 1) / (2 * kChannels);
-  const int64_t groups = a->rows < a->num_groups ? a->rows : a->num_groups;   // groups that can have rows
-  const int64_t mean = (a->rows + groups - 1) / groups;
-  int t = mean <= 16 ? 64 : mean <= 64 ? 128 : 256;
-  while (t > kMinRows && groups * ((mean + t / 2 - 1) / (t / 2)) * tiles_n <= pairs()) t /= 2;
-  return t;
-}
-
-// Bytes of workspace with which the tiles of a partial wave can be split; 0 where that does not pay: with larger tiles (the parts
-// of 128 rows cost more than the idle pairs: 300 rows, K = 14336: 54 us against 46), a short contraction or many waves.
-size_t workspace_bytes(const fp8gmm_int8_gemm_args* a, int tile_rows) {
-  if (a->rows <= 0 || a->num_groups <= 0 || g_split == 0 || tile_rows != kMinRows) return 0;
   const int64_t groups = a->rows < a->num_groups ? a->rows : a->num_groups;
-  const int64_t tiles = (a->rows / tile_rows + groups) * ((a->n + 2 * kChannels - 1) / (2 * kChannels));
-  if (tiles > 8 * static_cast<int64_t>(pairs()) || a->k <= kBlockK * Schedule::kMinGain) return 0;
-  return kCounterBytes + static_cast<size_t>(pairs()) * 4 * tile_rows * kChannels * sizeof(int);
+  const int64_t mean = (a->rows + groups - 1) / groups;
+  return mean <= 64 || groups * ((mean + 127) / 128) * tiles_n <= pairs() ? 128 : 256;
 }
 
 }  // namespace
@@ -563,7 +442,6 @@ int int8_gemm_check(const fp8gmm_int8_gemm_args* a) {
   FP8GMM_CHECK_ARG(a->a && a->b && a->c && a->a_scales && a->b_scales, "int8_grouped_gemm: NULL pointer");
   FP8GMM_CHECK_ARG((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->b) | reinterpret_cast<uintptr_t>(a->c)) % 16 == 0,
                    "int8_grouped_gemm: operand pointers must be 16-byte aligned");
-  FP8GMM_CHECK_ARG(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "int8_grouped_gemm: the workspace must be 16-byte aligned");
   return FP8GMM_OK;
 }
 
@@ -588,8 +466,8 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
   p.tile_rows = tile_rows;
   rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, kChannels);
   if (rc != FP8GMM_OK) return rc;
-  for (int i = 0; i < 3 && 64 << i <= tile_rows; ++i) {
-    rc = encode_rows(&p.map_x[i], a->a, a->rows, a->k, 32 << i);
+  for (; p.x_maps < 4 && (p.x_maps == 0 || (32 << p.x_maps <= tile_rows && 16 << p.x_maps < p.rows)); ++p.x_maps) {
+    rc = encode_rows(&p.map_x[p.x_maps], a->a, a->rows, a->k, 16 << p.x_maps);
     if (rc != FP8GMM_OK) return rc;
   }
   p.stage_bytes = kWBytes + tile_rows / 2 * kBlockK;
@@ -601,15 +479,7 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
   const int64_t most = (p.rows / tile_rows + (p.rows < p.num_groups ? p.rows : p.num_groups)) * static_cast<int64_t>(p.tiles_n);
   FP8GMM_CHECK_ARG(most <= INT32_MAX / 2, "int8_grouped_gemm: problem too large");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const size_t want = workspace_bytes(a, tile_rows);
-  int workers = pairs();
-  if (want > 0 && a->workspace != nullptr && a->workspace_bytes >= want) {
-    p.counters = static_cast<unsigned int*>(a->workspace);
-    p.parts = reinterpret_cast<int*>(static_cast<char*>(a->workspace) + kCounterBytes);
-    if (!after_quantize) FP8GMM_CHECK_CUDA(cudaMemsetAsync(p.counters, 0, kCounterBytes, s));
-  } else if (most < workers) {
-    workers = static_cast<int>(most);
-  }
+  const int workers = most < pairs() ? static_cast<int>(most) : pairs();
   rc = allow_shared_memory();
   if (rc != FP8GMM_OK) return rc;
   FP8GMM_CHECK_CUDA(launch_dependent(int8_gemm_kernel, 2 * workers, kThreads, kSmemBytes, s, after_quantize, p));
@@ -621,19 +491,11 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
 
 extern "C" {
 
-int fp8gmm_set_int8_variant(int tile_rows, int split) {
+int fp8gmm_set_int8_variant(int tile_rows) {
   using namespace fp8gmm;
-  FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 64 || tile_rows == 128 || tile_rows == 256,
-                   "set_int8_variant: tile_rows must be 0, 64, 128 or 256");
+  FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 128 || tile_rows == 256, "set_int8_variant: tile_rows must be 0, 128 or 256");
   g_tile_rows = tile_rows;
-  g_split = split != 0;
   return FP8GMM_OK;
-}
-
-size_t fp8gmm_int8_workspace_bytes(const fp8gmm_int8_gemm_args* a) {
-  using namespace fp8gmm;
-  if (a == nullptr || a->rows <= 0 || a->num_groups <= 0) return 0;
-  return workspace_bytes(a, choose_tile_rows(a));
 }
 
 int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) { return fp8gmm::int8_gemm_launch(a, stream, false); }
@@ -644,8 +506,7 @@ int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gem
                    "int8_linear: the product has to take the codes, scales, rows and columns of the quantisation");
   int rc = fp8gmm::int8_gemm_check(g);   // before anything is launched
   if (rc != FP8GMM_OK) return rc;
-  // the quantisation zeroes the counters that the product's split tiles need
-  rc = fp8gmm::quantize_rows_launch(q, g->workspace_bytes >= fp8gmm::kCounterBytes ? g->workspace : nullptr, fp8gmm::kCounterBytes / 4, stream);
+  rc = fp8gmm_quantize_rows_int8(q, stream);
   return rc != FP8GMM_OK ? rc : fp8gmm::int8_gemm_launch(g, stream, q->rows > 0);
 }
 

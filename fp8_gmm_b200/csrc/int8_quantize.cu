@@ -35,8 +35,6 @@ struct QuantRowsParams {
   int8_t* codes;
   float* scales;
   int* status;
-  uint32_t* zero;      // words to be zeroed for the kernel behind this one, or NULL
-  int zero_words;
 };
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
@@ -103,11 +101,6 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* warp_max) {
   return __reduce_max_sync(0xFFFFFFFFu, lane < warps ? warp_max[lane] : 0u);
 }
 
-__device__ __forceinline__ void zero_words(const QuantRowsParams& p) {
-  if (p.zero != nullptr && blockIdx.x == 0 && threadIdx.y == 0)
-    for (int i = threadIdx.x; i < p.zero_words; i += blockDim.x) p.zero[i] = 0u;
-}
-
 // Source row of row r, or -1 (reported) if the index names none.
 __device__ __forceinline__ int64_t source_row(const QuantRowsParams& p, int64_t r) {
   if (p.indices == nullptr) return r;
@@ -122,7 +115,6 @@ template <int kAct, int kVecs>
 __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_ACT_SWIGLU ? 2 : 3) quantize_rows_kernel(const QuantRowsParams p) {
   __shared__ uint32_t warp_max[kMaxThreads / 32];
   let_dependents_start();
-  zero_words(p);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const bool live = r < p.rows;
   const int64_t src = live ? source_row(p, r) : -1;
@@ -175,7 +167,6 @@ template <int kAct>
 __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const QuantRowsParams p) {
   __shared__ uint32_t warp_max[2][kLongThreads / 32];
   let_dependents_start();
-  zero_words(p);
   int turn = 0;   // two sets of places: a warp may be one row ahead of another
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
     const int64_t src = source_row(p, r);
@@ -221,8 +212,12 @@ void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
 }
 
 }  // namespace
+}  // namespace fp8gmm
 
-int quantize_rows_launch(const fp8gmm_quantize_rows_args* a, void* zero, int zero_words, void* stream) {
+extern "C" {
+
+int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) {
+  using namespace fp8gmm;
   FP8GMM_CHECK_ARG(a != nullptr, "quantize_rows_int8: NULL arguments");
   FP8GMM_CHECK_ARG(a->rows >= 0 && a->cols >= 0 && a->in_rows >= 0, "quantize_rows_int8: negative size");
   FP8GMM_CHECK_ARG(a->activation == FP8GMM_ACT_NONE || a->activation == FP8GMM_ACT_GELU || a->activation == FP8GMM_ACT_SWIGLU,
@@ -244,8 +239,6 @@ int quantize_rows_launch(const fp8gmm_quantize_rows_args* a, void* zero, int zer
   p.cols = a->cols;
   p.codes = static_cast<int8_t*>(a->codes);
   p.scales = a->scales;
-  p.zero = static_cast<uint32_t*>(zero);
-  p.zero_words = zero_words;
   p.status = device_status_word();
   FP8GMM_CHECK_ARG(p.status != nullptr, "quantize_rows_int8: cannot resolve the device status word");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -255,14 +248,6 @@ int quantize_rows_launch(const fp8gmm_quantize_rows_args* a, void* zero, int zer
   FP8GMM_CHECK_CUDA(cudaGetLastError());
   count_launch();
   return FP8GMM_OK;
-}
-
-}  // namespace fp8gmm
-
-extern "C" {
-
-int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) {
-  return fp8gmm::quantize_rows_launch(a, nullptr, 0, stream);
 }
 
 }  // extern "C"

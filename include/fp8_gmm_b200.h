@@ -453,13 +453,7 @@ typedef struct {
   int64_t rows;
   int64_t n;
   int64_t k;
-  void* workspace;         /* optional device memory, 16-byte aligned, for this call alone until it has run: with
-                              fp8gmm_int8_workspace_bytes(args) bytes the tiles of a partial wave are split along K */
-  size_t workspace_bytes;
 } fp8gmm_int8_gemm_args;
-
-/* Workspace that the call can make use of; 0 where it would not help. */
-size_t fp8gmm_int8_workspace_bytes(const fp8gmm_int8_gemm_args* args);
 
 int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
 
@@ -467,9 +461,9 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
  * rows and columns); the product starts loading weights while the rows are still being quantised. */
 int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gemm_args* g, void* stream);
 
-/* Process-wide switch of the launches above, for tests and experiments: rows of a tile (64, 128 or 256; 0 = chosen per call,
- * the default) and whether the tiles of a partial wave may be split along K (default 1).  Results are bit-identical. */
-int fp8gmm_set_int8_variant(int tile_rows, int split);
+/* Process-wide switch of the launches above, for tests and experiments: rows of a tile (128 or 256; 0 = chosen per call, the
+ * default).  Results are bit-identical. */
+int fp8gmm_set_int8_variant(int tile_rows);
 
 /* ------------------------------------------------------------------------------------------------
  * Global 2-norm of a list of gradients, and clipping by it: what stands between the weight gradients and the optimizer.
