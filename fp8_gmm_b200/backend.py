@@ -9,9 +9,11 @@ List-style ops accept any number of tensors per call (the reference stops at 64)
 functions are the allocation-free fast forms the modules use: one base tensor plus host prefix sums
 instead of Python lists of per-group views.
 """
+import array
 import contextlib
 import ctypes
 import math
+import operator
 import os
 
 import numpy as np
@@ -683,7 +685,7 @@ def _quantize_args(x, indices, top_k, activation):
     if indices is not None:
         if not (indices.dtype == torch.int32 and indices.device == x.device and indices.dim() == 1 and indices.is_contiguous()):
             _fail("quantize_rows_int8: indices must be a contiguous 1-D CUDA int32 tensor on the device of x")
-        if top_k < 1:
+        if not 1 <= top_k < 2 ** 31:
             _fail("quantize_rows_int8: top_k must be positive")
         lead = indices.shape
         args.indices, args.top_k, args.rows = indices.data_ptr(), int(top_k), lead[0]
@@ -823,31 +825,43 @@ def _check_grads(grads, outputs, name):
             o = outputs[i]
             if not o.is_cuda or o.get_device() != index or o.dtype not in _GRAD_TYPE:
                 _fail(f"{name}: output {i} must be a bfloat16, float16 or float32 tensor on the device of the gradients")
-            if o.shape != g.shape or not (g.is_contiguous() and o.is_contiguous() or o.stride() == g.stride()):
+            if not (g.is_contiguous() and o.is_contiguous() and o.numel() == g.numel() or o.shape == g.shape and o.stride() == g.stride()):
                 _fail(f"{name}: output {i} does not have the layout of its gradient")
+
+
+# unbound, for map() over lists of gradients: about 0.6 us a tensor and its output in all, half of what a loop takes
+_DATA_PTR, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.numel
+_IS_CONTIGUOUS, _GET_DEVICE, _DTYPE = torch.Tensor.is_contiguous, torch.Tensor.get_device, operator.attrgetter("dtype")
 
 
 def _kinds(tensors, index):
     """Type codes of the tensors if all are contiguous ones of the kernels' types on the CUDA device ``index``, else None."""
-    kinds = [_GRAD_TYPE.get(t.dtype) for t in tensors]
-    if index < 0 or None in kinds or not all([t.get_device() == index and t.is_contiguous() for t in tensors]):
+    kinds = list(map(_GRAD_TYPE.get, map(_DTYPE, tensors)))
+    if index < 0 or None in kinds or set(map(_GET_DEVICE, tensors)) != {index} or not all(map(_IS_CONTIGUOUS, tensors)):
         return None
     return kinds
 
 
 def _grad_descs(grads, outputs, name):
     """Descriptor array (fp8gmm_grad_desc: in, out, numel, in_type | out_type << 32) and the common device."""
-    if outputs is not None and len(outputs) != len(grads):
+    outs = grads if outputs is None else list(outputs)
+    if len(outs) != len(grads):
         _fail(f"{name}: one output per gradient is required")
     index = grads[0].get_device()
     kinds = _kinds(grads, index)
-    out_kinds = kinds if outputs is None else _kinds(outputs, index)
-    if kinds is None or out_kinds is None or outputs is not None and any([g.shape != o.shape for g, o in zip(grads, outputs)]):
-        _check_grads(grads, outputs, name)   # the slow way round: permuted dense tensors, or what is wrong
+    out_kinds = kinds if outputs is None else _kinds(outs, index)
+    numels = list(map(_NUMEL, grads))
+    if kinds is None or out_kinds is None or outputs is not None and list(map(_NUMEL, outs)) != numels:
+        _check_grads(grads, None if outputs is None else outs, name)   # permuted dense tensors, or something is wrong
         kinds = [_GRAD_TYPE[g.dtype] for g in grads]
-        out_kinds = kinds if outputs is None else [_GRAD_TYPE[o.dtype] for o in outputs]
-    rows = [v for g, o, k, ok in zip(grads, outputs or grads, kinds, out_kinds) for v in (g.data_ptr(), o.data_ptr(), g.numel(), k | ok << 32)]
-    return (ctypes.c_int64 * len(rows))(*rows), grads[0].device
+        out_kinds = [_GRAD_TYPE[o.dtype] for o in outs]
+    rows = [0] * (4 * len(grads))
+    rows[0::4] = rows[1::4] = list(map(_DATA_PTR, grads))
+    if outputs is not None:
+        rows[1::4] = map(_DATA_PTR, outs)
+    rows[2::4] = numels
+    rows[3::4] = [k | o << 32 for k, o in zip(kinds, out_kinds)]
+    return array.array("q", rows), grads[0].device
 
 
 def _grad_workspace(count, device):
@@ -865,7 +879,7 @@ def multi_sum_squares(grads):
     descs, device = _grad_descs(grads, None, "multi_sum_squares")
     with _on(device):
         ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_sum_squares(descs, len(grads), ws.data_ptr(), ws.numel() * 8, out.data_ptr(), None, _stream()),
+        check(lib.fp8gmm_multi_sum_squares(descs.buffer_info()[0], len(grads), ws.data_ptr(), ws.numel() * 8, out.data_ptr(), None, _stream()),
               "multi_sum_squares")
     return out
 
@@ -879,7 +893,7 @@ def multi_grad_norm(grads):
     descs, device = _grad_descs(grads, None, "multi_grad_norm")
     with _on(device):
         ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_sum_squares(descs, len(grads), ws.data_ptr(), ws.numel() * 8, None, out.data_ptr(), _stream()),
+        check(lib.fp8gmm_multi_sum_squares(descs.buffer_info()[0], len(grads), ws.data_ptr(), ws.numel() * 8, None, out.data_ptr(), _stream()),
               "multi_grad_norm")
     return out
 
@@ -891,17 +905,18 @@ def _max_norm(value, name):
 
 
 def multi_clip(grads, sum_squares, max_norm, outputs=None):
-    """Scales every gradient by ``min(1, max_norm / (sqrt(sum_squares) + 1e-6))``, in place or into ``outputs`` (which may
-    have another float type: bf16 gradients into an optimizer's fp32 ones).  ``sum_squares``: 0-dim float64 CUDA tensor
+    """Scales every gradient by ``min(1, max_norm / (sqrt(sum_squares) + 1e-6))``, in place or into ``outputs``, which may have
+    another float type, and another shape if both are contiguous: bf16 gradients into pieces of an optimizer's flat fp32
+    buffer.  ``sum_squares``: 0-dim float64 CUDA tensor
     (``multi_sum_squares``).  Returns its square root, 0-dim float32; a NaN there makes every output NaN."""
     grads = list(grads)
     _require(sum_squares.is_cuda and sum_squares.dtype == torch.float64 and sum_squares.numel() == 1, "multi_clip: sum_squares must be one CUDA float64 value")
     max_norm = _max_norm(max_norm, "multi_clip")
     norm = torch.empty((), dtype=torch.float32, device=sum_squares.device)
-    descs, device = _grad_descs(grads, outputs, "multi_clip") if grads else ((ctypes.c_int64 * 0)(), sum_squares.device)
+    descs, device = _grad_descs(grads, outputs, "multi_clip") if grads else (array.array("q"), sum_squares.device)
     _require(device == sum_squares.device, "multi_clip: sum_squares is on another device than the gradients")
     with _on(device):
-        check(lib.fp8gmm_multi_clip(descs, len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr(), _stream()), "multi_clip")
+        check(lib.fp8gmm_multi_clip(descs.buffer_info()[0], len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr(), _stream()), "multi_clip")
     return norm
 
 
@@ -916,7 +931,7 @@ def multi_clip_grad_norm(grads, max_norm, outputs=None):
     descs, device = _grad_descs(grads, outputs, "multi_clip_grad_norm")
     with _on(device):
         ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_clip_grad_norm(descs, len(grads), max_norm, ws.data_ptr(), ws.numel() * 8, norm.data_ptr(), _stream()),
+        check(lib.fp8gmm_multi_clip_grad_norm(descs.buffer_info()[0], len(grads), max_norm, ws.data_ptr(), ws.numel() * 8, norm.data_ptr(), _stream()),
               "multi_clip_grad_norm")
     return norm
 

@@ -16,6 +16,7 @@ namespace fp8gmm {
 void set_error(const char* fmt, ...);
 int cuda_fail(cudaError_t err, const char* what);
 int sm_count();              // SMs of the current device (cached per device)
+int gemm_sms();              // of these, how many the persistent GEMM kernels may occupy (fp8gmm_set_gemm_sm_limit)
 int* device_status_word();   // device address of the per-device status word (kernels report timeouts here)
 void count_launch();         // bumps the process-wide launch counter (fp8gmm_launch_count)
 unsigned long long gemm_wait_limit_ns();  // limit of the GEMM kernels' mbarrier waits (fp8gmm_set_wait_limits)

@@ -916,6 +916,14 @@ uint32_t make_idesc(int a_format, int b_format, int ctas, bool a_mn = false, boo
 // Upper bound on the SMs a GEMM launch occupies (fp8gmm_set_gemm_sm_limit; 0 = all).  A persistent grid that
 // fills every SM is delayed as a whole when another kernel (an NCCL exchange on a second stream) holds a few SMs.
 int g_sm_limit = 0;
+}  // namespace
+
+int gemm_sms() {
+  const int sms = sm_count();
+  return g_sm_limit > 0 && g_sm_limit < sms ? g_sm_limit : sms;
+}
+
+namespace {
 
 // Wave counters of the long-contraction launches: a small ring of words in device memory, one per launch in flight.
 constexpr int kWaveSlots = 64;
@@ -946,8 +954,7 @@ unsigned int* next_wave_counter(cudaStream_t s) {
 
 int launch(GemmParams& p, int ctas, cudaStream_t s) {
   // The attribute is per device and the call is idempotent and cheap, so it is simply repeated.
-  int sms = sm_count();
-  if (g_sm_limit > 0 && g_sm_limit < sms) sms = g_sm_limit;
+  const int sms = gemm_sms();
   const int workers = sms / ctas > 0 ? sms / ctas : 1;
   const int grid = ctas * (p.total_tiles < workers ? p.total_tiles : workers);
   p.wait_ns = gemm_wait_limit_ns();

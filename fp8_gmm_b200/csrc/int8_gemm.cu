@@ -400,7 +400,7 @@ int allow_shared_memory() {
   return FP8GMM_OK;
 }
 
-int pairs() { return sm_count() / 2; }
+int pairs() { return gemm_sms() > 1 ? gemm_sms() / 2 : 1; }
 
 // Rows of a tile: 256, which reads the weights least often, or 128 for groups of up to 64 rows (two more stages in flight) and where
 // smaller tiles still fit one wave of the grid.  It goes by the mean rows of a group that can have any, so that sizes on the
