@@ -129,7 +129,7 @@ SYMBOLS = {
     "fp8gmm_quantize_rows_int8": (ctypes.c_int, [ctypes.POINTER(QuantizeRowsArgs), c_vp]),
     "fp8gmm_int8_grouped_gemm": (ctypes.c_int, [ctypes.POINTER(Int8GemmArgs), c_vp]),
     "fp8gmm_int8_linear": (ctypes.c_int, [ctypes.POINTER(QuantizeRowsArgs), ctypes.POINTER(Int8GemmArgs), c_vp]),
-    "fp8gmm_set_int8_variant": (ctypes.c_int, [ctypes.c_int]),
+    "fp8gmm_set_int8_variant": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
     "fp8gmm_sum_squares_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int]),
     "fp8gmm_multi_sum_squares": (ctypes.c_int, [c_vp, ctypes.c_int, c_vp, ctypes.c_size_t, c_vp, c_fp, c_vp]),
     "fp8gmm_multi_clip": (ctypes.c_int, [c_vp, ctypes.c_int, c_vp, ctypes.c_float, c_fp, c_vp]),

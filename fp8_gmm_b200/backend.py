@@ -77,10 +77,10 @@ def set_gemm_variant(ctas=0, tail_split=True, tma_epilogue=True):
     check(lib.fp8gmm_set_gemm_variant(int(ctas), int(bool(tail_split)), int(bool(tma_epilogue))), "set_gemm_variant")
 
 
-def set_int8_variant(tile_rows=0):
-    """Force the rows of the int8 product's tiles (128 or 256; 0 = automatic); see fp8gmm_set_int8_variant.  For tests and
-    experiments: results are bit-identical."""
-    check(lib.fp8gmm_set_int8_variant(int(tile_rows)), "set_int8_variant")
+def set_int8_variant(tile_rows=0, tile_channels=0):
+    """Force the rows and channels of the int8 product's tiles (128 or 256 each; 0 = automatic); see fp8gmm_set_int8_variant.
+    For tests and experiments: results are bit-identical."""
+    check(lib.fp8gmm_set_int8_variant(int(tile_rows), int(tile_channels)), "set_int8_variant")
 
 
 def set_wait_limits(gemm_wait_s=0.0, peer_wait_s=0.0):

@@ -9,8 +9,10 @@
 // The operands are swapped against gemm_sm100.cu: output channels are the M dimension of the MMA (TMEM lanes), rows the N
 // dimension (TMEM columns).  A group of any number of rows then costs an MMA only as wide as its rows, and a warp's 32 lanes
 // hold 32 neighbouring channels of one output row.
-//   * Persistent CTA pairs (cta_group::2): a tile is 256 channels x up to 128 or 256 rows; each CTA loads its 128 channels of
-//     weights and half of the tile's rows, 128 contraction bytes per stage, into a ring of 8 or 6 stages.
+//   * Persistent CTA pairs (cta_group::2): a tile is 256 channels x up to 128 or 256 rows; each CTA loads its half of the channels'
+//     weights and half of the tile's rows, 256 contraction bytes per stage, into a ring of 4 or 3 stages.  Where such tiles would
+//     keep less than half of the GPU loading weights (few experts, few channels, few rows), a tile is 128 channels: the MMA stays
+//     256 wide and its other rows, whatever lies in shared memory behind the weights, are not looked at.
 //   * Accumulators are double-buffered in TMEM; results are transposed through shared memory and written as 256-byte runs.
 // Group sizes come from the host (parameter block) or are read on the device; either way every CTA builds the prefix sums of
 // rows and tiles in shared memory.  Waits on mbarriers are bounded as in gemm_sm100.cu.
@@ -26,12 +28,13 @@ namespace {
 constexpr int kMaxGroups = 512;
 constexpr int kStatusBadSizes = 0x400;   // group sizes that are negative or reach behind the last row
 constexpr int kThreads = 192;            // TMA producer warp, MMA warp, four epilogue warps
-constexpr int kChannels = 128;           // channels of one CTA's tile
-constexpr int kBlockK = 128;             // bytes of contraction per stage: one 128-byte swizzle atom
-constexpr int kWBytes = kChannels * kBlockK;
+constexpr int kChannels = 128;           // channels of one CTA's half of the MMA
+constexpr int kAtomK = 128;              // bytes of contraction in one box: a 128-byte swizzle atom
+constexpr int kAtoms = 2;                // boxes along the contraction per stage
+constexpr int kBlockK = kAtoms * kAtomK;
 
 struct Int8GemmParams {
-  CUtensorMap map_w;                     // weights (G*N, K), box 128 rows x 128 bytes
+  CUtensorMap map_w;                     // weights (G*N, K), box of `channels` rows x 128 bytes
   CUtensorMap map_x[4];                  // codes (rows, K), boxes of 16, 32, 64 and 128 rows x 128 bytes (up to half of tile_rows): a
                                          // tile with few rows loads no more than it needs
   uint16_t* c;
@@ -41,6 +44,7 @@ struct Int8GemmParams {
   int* status;
   unsigned long long wait_ns;
   int num_groups, rows, n, k;
+  int channels;                          // of one CTA's half of a tile: 128 or 64
   int tile_rows, tiles_n, super_tiles;
   int x_maps;                            // entries of map_x that a tile can need
   int stages, stage_bytes;
@@ -129,14 +133,14 @@ __device__ __forceinline__ Tile decode_tile(const Int8GemmParams& p, const int* 
   const int h = min(p.super_tiles, row_tiles - s * p.super_tiles);
   const int mt = s * p.super_tiles + rem % h;
   t.group = g;
-  t.n0 = rem / h * (2 * kChannels);
+  t.n0 = rem / h * (2 * p.channels);
   t.row0 = row_start[g] + mt * p.tile_rows;
   t.rows = min(p.tile_rows, m - mt * p.tile_rows);
   return t;
 }
 
 constexpr int kMaxRows = 256;                 // rows of the larger tile
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 12 / kAtoms;
 constexpr int kRingBytes = 6 * 32 * 1024;
 constexpr int kTmemCols = 512;
 constexpr int kBoxBytes = 32 * kChannels * 2; // 32 rows x 128 channels of bf16
@@ -177,7 +181,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const bool leader = rank == 0;
-  const int stages = p.stages, stage_bytes = p.stage_bytes;
+  const int stages = p.stages, stage_bytes = p.stage_bytes, w_bytes = p.channels * kAtomK, x_bytes = p.tile_rows / 2 * kAtomK;
 
   if (threadIdx.x == 32) {
     for (int s = 0; s < stages; ++s) {
@@ -210,7 +214,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
   if (warp == 0) {
     // ===================== TMA producer: both CTAs credit the leader's barriers =====================
     // The whole warp walks the loop and one elected lane issues: code under a test of the lane number cannot keep its operands in
-    // uniform registers, and the MMA warp's loop took 300 ns a K block that way instead of 200 (one tile of 256 x 1).
+    // uniform registers, and the MMA warp's loop took 300 ns per 128 bytes of contraction that way instead of 190 (one tile of 256
+    // channels and few rows).  Waiting for barriers and signalling them accounts for most of that, so a stage is two boxes deep: 97 ns.
     const bool issue = elect_one();
     int stage = 0;
     uint32_t phase = 0;
@@ -219,21 +224,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     for (int tile = worker; tile < total_tiles && ok; tile += num_workers) {
       const Tile t = decode_tile(p, row_start, tile_start, tile);
       const int width = mma_width(t.rows);
-      const int yw = t.group * p.n + t.n0 + rank * kChannels, yx = t.row0 + rank * (width / 2);
+      const int yw = t.group * p.n + t.n0 + rank * p.channels, yx = t.row0 + rank * (width / 2);
       const int box = width <= 32 ? 0 : width <= 64 ? 1 : width <= 128 ? 2 : 3;   // box of 16 << box rows: one CTA's half
       const CUtensorMap* map_x = &p.map_x[box];
-      const int bytes = 2 * (kWBytes + (16 << box) * kBlockK);                    // of both CTAs
+      const int bytes = 2 * kAtoms * (w_bytes + (16 << box) * kAtomK);                    // of both CTAs
       int kb = 0;
       if (tile == worker) {
         // Weights do not depend on the kernel before this one (the quantisation of the rows): a ring full of them goes ahead.
         const int first = min(num_kb, stages);
         for (int i = 0; i < first; ++i) {
           if (leader && issue) mbar_expect_tx(full_bar(i), bytes);
-          if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes, &p.map_w, full0_leader + 8u * i, i * kBlockK, yw);
+#pragma unroll
+          for (int h = 0; h < kAtoms; ++h)
+            if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes + h * w_bytes, &p.map_w, full0_leader + 8u * i, i * kBlockK + h * kAtomK, yw);
         }
         grid_dependency_wait();
         for (int i = 0; i < first; ++i)
-          if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes + kWBytes, map_x, full0_leader + 8u * i, i * kBlockK, yx);
+#pragma unroll
+          for (int h = 0; h < kAtoms; ++h)
+            if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes + kAtoms * w_bytes + h * x_bytes, map_x, full0_leader + 8u * i, i * kBlockK + h * kAtomK, yx);
         kb = first;
         stage = first == stages ? 0 : first;
         phase = first == stages ? 1u : 0u;
@@ -243,8 +252,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
         if (ok) {
           const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
           if (leader && issue) mbar_expect_tx(full_bar(stage), bytes);
-          if (issue) tma_load_2d_pair(sw, &p.map_w, bar, kb * kBlockK, yw);
-          if (issue) tma_load_2d_pair(sw + kWBytes, map_x, bar, kb * kBlockK, yx);
+#pragma unroll
+          for (int h = 0; h < kAtoms; ++h) {
+            if (issue) tma_load_2d_pair(sw + h * w_bytes, &p.map_w, bar, kb * kBlockK + h * kAtomK, yw);
+            if (issue) tma_load_2d_pair(sw + kAtoms * w_bytes + h * x_bytes, map_x, bar, kb * kBlockK + h * kAtomK, yx);
+          }
         }
         if (++stage == stages) {
           stage = 0;
@@ -257,7 +269,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     // ===================== MMA issuer: one lane of the leader =====================
     if (leader) {
       const bool issue = elect_one();
-      const uint64_t desc_w0 = make_smem_desc(tiles_addr), desc_x0 = make_smem_desc(tiles_addr + kWBytes);
+      const uint64_t desc_w0 = make_smem_desc(tiles_addr), desc_x0 = make_smem_desc(tiles_addr + kAtoms * w_bytes);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -275,7 +287,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
           const uint64_t dx = desc_x0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
 #pragma unroll
           for (int k = 0; k < kBlockK / 32; ++k)
-            if (issue) umma_i8_pair(tmem_d, dw + 2 * k, dx + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            if (issue)
+              umma_i8_pair(tmem_d, dw + (k >> 2) * (w_bytes >> 4) + 2 * (k & 3), dx + (k >> 2) * (x_bytes >> 4) + 2 * (k & 3), idesc, (kb | k) != 0 ? 1u : 0u);
           if (issue) umma_commit_pair(empty_bar(stage));
           if (++stage == stages) {
             stage = 0;
@@ -299,9 +312,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     grid_dependency_wait();
     for (int tile = worker; tile < total_tiles; tile += num_workers) {
       const Tile t = decode_tile(p, row_start, tile_start, tile);
-      const int n0 = t.n0 + rank * kChannels;
+      const int n0 = t.n0 + rank * p.channels;
+      const int n_end = min(n0 + p.channels, p.n);
       const int channel = n0 + quad * 32 + lane;
-      const float sb = channel < p.n ? p.b_scales[static_cast<int64_t>(t.group) * p.n + channel] : 0.f;
+      const float sb = channel < n_end ? p.b_scales[static_cast<int64_t>(t.group) * p.n + channel] : 0.f;
       float* scales = scale_buf + acc * kMaxRows;
       for (int i = thread; i < t.rows; i += 128) scales[i] = p.a_scales[t.row0 + i];
       if (lane == 0 && ok) ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 0x8, p.wait_ns);
@@ -329,7 +343,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
         epilogue_barrier();
         // 16 threads write the 256 bytes of a row; the box is free again after the next barrier
         const int chunk = thread & 15;
-        if (ok && n0 + chunk * 8 < p.n) {
+        if (ok && n0 + chunk * 8 < n_end) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = i * 8 + (thread >> 4);
@@ -373,7 +387,7 @@ int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, 
   }
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
-  const cuuint32_t box[2] = {kBlockK, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t box[2] = {kAtomK, static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -386,7 +400,7 @@ int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, 
 }
 
 // Process-wide override for tests (fp8gmm_set_int8_variant): 0 = chosen per call.
-int g_tile_rows = 0;
+int g_tile_rows = 0, g_channels = 0;
 
 // Once per device: the attribute stays.
 int allow_shared_memory() {
@@ -402,19 +416,27 @@ int allow_shared_memory() {
 
 int pairs() { return gemm_sms() > 1 ? gemm_sms() / 2 : 1; }
 
-// Rows of a tile: 256, which reads the weights least often, or 128 for groups of up to 64 rows (two more stages in flight) and where
-// smaller tiles still fit one wave of the grid.  It goes by the mean rows of a group that can have any, so that sizes on the
-// host and on the device take the same tile.  Measured, product and quantisation, us (128 / 256 rows): eight experts of 4096 x
-// 4096 with 8 rows each 25.8 / 26.6, with 32 rows 29.5 / 30.0, with 64 rows 32.0 / 31.7, with 256 rows 49.4 / 47.0, with 1024 rows 138 / 117;
-// one expert of 1024 x 4096 with 1024 rows 15.4 / 20.3, of 4096 x 14336 with 300 rows 33.8 / 45.3.  (Tiles of 64 rows: 25.7 and
-// 14.9 at best.  Splitting the contraction of the tiles of a partial wave between pairs, with sums handed on through L2, cost about
-// 8 us a tile and paid only below 16 tiles: dropped.)
-int choose_tile_rows(const fp8gmm_int8_gemm_args* a) {
-  if (g_tile_rows != 0) return g_tile_rows;
+// Rows and channels of a tile.  256 rows read the weights least often; 128 are for groups of up to 128 rows (one more stage in
+// flight) and where smaller tiles still fit one wave of the grid; 128 channels where tiles of 256 would fill less than half of it
+// and the time goes into loading weights.  The rule goes by the mean rows of a group that can have any, so that sizes on the host
+// and on the device take the same tile.  Measured, product and quantisation, us.  128 / 256 rows: eight experts of 4096 x 4096
+// with 8 rows each 24.9 / 25.8, with 128 rows 35.4 / 37.1, with 256 rows 46.3 / 47.1, with 1024 rows 125 / 115; 64 experts of 1424 x 2048 with
+// 256 rows 88 / 82; one expert of 1024 x 4096 with 1024 rows 13.9 / 20.1, of 4096 x 14336 with 300 rows 30.0 / 44.2.  128 / 256 channels: one
+// row for each of two experts of 4096 x 14336 24.8 / 27.6, of 4096 x 4096 10.7 / 11.4; one expert of 4096 x 14336 with 16 rows 18.8 / 23.5, with 128 rows
+// 25.7 / 27.8, of 1024 x 4096 with 1024 rows 14.7 / 13.9.  (Splitting the contraction of a partial wave's tiles between pairs, with sums
+// handed on through L2, cost about 8 us a tile: dropped.)
+struct TileShape {
+  int rows, channels;
+};
+TileShape choose_tile(const fp8gmm_int8_gemm_args* a) {
   const int64_t tiles_n = (a->n + 2 * kChannels - 1) / (2 * kChannels);
   const int64_t groups = a->rows < a->num_groups ? a->rows : a->num_groups;
   const int64_t mean = (a->rows + groups - 1) / groups;
-  return mean <= 64 || groups * ((mean + 127) / 128) * tiles_n <= pairs() ? 128 : 256;
+  const int64_t small = groups * ((mean + 127) / 128) * tiles_n;   // tiles of 128 rows and 256 channels
+  TileShape t;
+  t.rows = g_tile_rows != 0 ? g_tile_rows : mean <= 128 || small <= pairs() ? 128 : 256;
+  t.channels = g_channels != 0 ? g_channels / 2 : mean <= 128 && 2 * small <= pairs() ? kChannels / 2 : kChannels;
+  return t;
 }
 
 }  // namespace
@@ -462,17 +484,19 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
   p.wait_ns = gemm_wait_limit_ns();
   p.status = device_status_word();
   FP8GMM_CHECK_ARG(p.status != nullptr, "int8_grouped_gemm: cannot resolve the device status word");
-  const int tile_rows = choose_tile_rows(a);
-  p.tile_rows = tile_rows;
-  rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, kChannels);
+  const TileShape tile = choose_tile(a);
+  const int tile_rows = p.tile_rows = tile.rows;
+  p.channels = tile.channels;
+  rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, p.channels);
   if (rc != FP8GMM_OK) return rc;
   for (; p.x_maps < 4 && (p.x_maps == 0 || (32 << p.x_maps <= tile_rows && 16 << p.x_maps < p.rows)); ++p.x_maps) {
     rc = encode_rows(&p.map_x[p.x_maps], a->a, a->rows, a->k, 16 << p.x_maps);
     if (rc != FP8GMM_OK) return rc;
   }
-  p.stage_bytes = kWBytes + tile_rows / 2 * kBlockK;
+  // with 64 channels the MMA reads 16 KiB from the start of each half of the weights all the same: into what lies behind them
+  p.stage_bytes = kAtoms * (p.channels + tile_rows / 2) * kAtomK;
   p.stages = kRingBytes / p.stage_bytes < kMaxStages ? kRingBytes / p.stage_bytes : kMaxStages;
-  p.tiles_n = (p.n + 2 * kChannels - 1) / (2 * kChannels);
+  p.tiles_n = (p.n + 2 * p.channels - 1) / (2 * p.channels);
   // a band of codes of 4096 rows (2048 with a long contraction) stays in L2 while the channel tiles sweep past it
   p.super_tiles = (p.k > 8192 ? 2048 : 4096) / tile_rows;
   // each group adds at most one partial row tile to rows / tile_rows
@@ -491,10 +515,12 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
 
 extern "C" {
 
-int fp8gmm_set_int8_variant(int tile_rows) {
+int fp8gmm_set_int8_variant(int tile_rows, int tile_channels) {
   using namespace fp8gmm;
   FP8GMM_CHECK_ARG(tile_rows == 0 || tile_rows == 128 || tile_rows == 256, "set_int8_variant: tile_rows must be 0, 128 or 256");
+  FP8GMM_CHECK_ARG(tile_channels == 0 || tile_channels == 128 || tile_channels == 256, "set_int8_variant: tile_channels must be 0, 128 or 256");
   g_tile_rows = tile_rows;
+  g_channels = tile_channels;
   return FP8GMM_OK;
 }
 

@@ -461,9 +461,9 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
  * rows and columns); the product starts loading weights while the rows are still being quantised. */
 int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gemm_args* g, void* stream);
 
-/* Process-wide switch of the launches above, for tests and experiments: rows of a tile (128 or 256; 0 = chosen per call, the
- * default).  Results are bit-identical. */
-int fp8gmm_set_int8_variant(int tile_rows);
+/* Process-wide switch of the launches above, for tests and experiments: rows and channels of a tile (128 or 256 each; 0 = chosen
+ * per call, the default).  Results are bit-identical. */
+int fp8gmm_set_int8_variant(int tile_rows, int tile_channels);
 
 /* ------------------------------------------------------------------------------------------------
  * Global 2-norm of a list of gradients, and clipping by it: what stands between the weight gradients and the optimizer.

@@ -171,11 +171,12 @@ def any_variant():
     backend.set_int8_variant()
 
 
+@pytest.mark.parametrize("tile_channels", [128, 256])
 @pytest.mark.parametrize("tile_rows", [128, 256])
-def test_every_tile_gives_the_same_bits(cuda, any_variant, tile_rows):
+def test_every_tile_gives_the_same_bits(cuda, any_variant, tile_rows, tile_channels):
     from fp8_gmm_b200 import backend
 
-    any_variant(tile_rows)
+    any_variant(tile_rows, tile_channels)
     for sizes, n, k in [([1], 16, 16), ([5, 0, 16, 17, 33], 272, 1040), ([64, 129, 1, 255, 256, 257], 400, 2080), ([2, 7], 1424, 4112), ([300], 128, 128),
                         ([300], 128, 8192), ([7, 0, 270], 272, 14336), ([3], 48, 131056), ([40] * 20, 1040, 2064)]:
         rows, G = sum(sizes), len(sizes)
