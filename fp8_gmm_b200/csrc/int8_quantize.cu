@@ -12,9 +12,9 @@
 // A row of zeros has scale 0 and codes 0.  A row that holds an infinity or a NaN has scale NaN and codes 0: all its products
 // come out NaN, no other row's do.
 //
-// Two kernels.  quantize_rows_kernel: a block for one row or several short ones, the row in registers between the maximum and the codes, so it is read
-// once; 16-byte loads, 8-byte stores.  quantize_long_rows_kernel: rows that are too long for that, or not aligned to 16 bytes,
-// are walked twice (the second time out of L2 or L1).
+// Two kernels.  quantize_rows_kernel: a block for one row or several short ones, the row in registers between the maximum and the
+// codes, so it is read once; 16-byte loads, 8-byte stores.  quantize_long_rows_kernel: rows that are too long for that, or not
+// aligned to 16 bytes, are walked twice (the second time out of L2 or L1).
 #include "int8.cuh"
 
 namespace fp8gmm {
@@ -39,13 +39,25 @@ struct QuantRowsParams {
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
 
-// The activation in fp32: hardware exp2 and division (a few ulp; their argument's rounding, |a| 2^-24, is larger from |a| = 4 on).
-// An exp that overflows gives a / inf = 0.
+// a / (1 + 2^p) from the hardware's exp2 and reciprocal, a few ulp (the rounding of exp2's argument, |p| 2^-24, is larger from
+// |p| = 4 on).  Both instructions flush subnormal numbers, so the quotient is taken 16 times as large, 16 / (1 + e) =
+// 1 / (1/16 + 2^(p - 4)): it then stays normal for every e = 2^p in fp32's range.  An exp that overflows gives 0.
+constexpr float kLog2E = 1.44269504f;
+__device__ __forceinline__ float over_one_plus_exp2(float a, float power_minus_4) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(power_minus_4));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 0.0625f));
+  return a * 0.0625f * r;
+}
 template <int kAct>
 __device__ __forceinline__ float activated(float a, float b) {
-  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return __fdividef(a, 1.f + __expf(-a)) * b;
-  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)): without the cancellation of 1 + tanh u at negative u
-  if constexpr (kAct == FP8GMM_ACT_GELU) return __fdividef(a, 1.f + __expf(-2.f * 0.79788456f * a * (1.f + 0.044715f * a * a)));
+  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return over_one_plus_exp2(a, fmaf(a, -kLog2E, -4.f)) * b;
+  if constexpr (kAct == FP8GMM_ACT_GELU) {
+    // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), without the cancellation of 1 + tanh u at
+    // negative u; the power of two is -2u log2(e) = a (c + 0.044715 c a^2)
+    constexpr float kC = -2.f * 0.79788456f * kLog2E;
+    return over_one_plus_exp2(a, fmaf(a, fmaf(a * a, 0.044715f * kC, kC), -4.f));
+  }
   return a;
 }
 
@@ -72,12 +84,12 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
   return s;
 }
 // The code in the low byte: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.  Behind
-// an activation there are no exact ties to respect (v itself is rounded), and one fused multiply-add does it.
+// an activation there are no exact ties to respect (v itself is rounded), and the quotient is not corrected.
 template <int kAct>
 __device__ __forceinline__ uint32_t code_of(float v, const RowScale& s) {
   constexpr float kMagic = 12582912.f;
-  if constexpr (kAct != FP8GMM_ACT_NONE) return __float_as_uint(fmaf(v, s.pre * s.inv, kMagic));
   const float t = v * s.pre;
+  if constexpr (kAct != FP8GMM_ACT_NONE) return __float_as_uint(fmaf(t, s.inv, kMagic));
   float y = t * s.inv;
   y = fmaf(fmaf(-y, s.top, t), s.inv, y);
   return __float_as_uint(y + kMagic);
@@ -194,10 +206,10 @@ void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
   const int64_t vecs = p.cols / 8;
   const bool aligned = p.cols % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
   if (aligned && vecs <= kMaxThreads * kMaxVecs && p.rows <= INT32_MAX) {
-    // Four vectors per thread keep more bytes in flight (measured against two: 32768 rows of 4096 70 / 81 us, behind SwiGLU
-    // 14336 wide 392 / 434 us = 6.0 TB/s); two answer sooner where all rows run at once, and fill a warp with a short row
+    // Four vectors per thread keep more bytes in flight (measured against two: 32768 rows of 4096 69 / 81 us, behind SwiGLU
+    // 14336 wide 384 / 434 us = 6.1 TB/s); two answer sooner where all rows run at once, and fill a warp with a short row
     // (100000 rows of 272: 29 / 37 us).  Short rows share a block, since starting a block takes about 1 ns of the GPU's
-    // time (one row per block: 262144 rows of 1024 took 272 us, now 129).
+    // time (one row per block: 262144 rows of 1024 took 272 us, now 126).
     const int per = vecs <= 64 || (vecs <= 2 * kMaxThreads && p.rows <= 4 * sm_count()) ? 2 : 4;
     const int threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
     const int rows_per_block = threads < 256 ? 256 / threads : 1;

@@ -105,6 +105,29 @@ def test_activation_far_out(cuda):
     assert q.cpu().tolist() == [[0, 127, 0, 1, 0]] and torch.isfinite(s).all()
 
 
+@pytest.mark.parametrize("act", ["gelu", "swiglu"])
+def test_activations_near_the_end_of_fp32s_range(cuda, act):
+    """Rows whose activations are all tiny: products near 1e-39, and gates at -88, where e^88 is within a factor of two of
+    fp32's largest number (subnormal activations keep at least 18 bits here, more than ACT_REL asks)."""
+    from fp8_gmm_b200 import backend
+
+    width = 40
+    g = torch.Generator().manual_seed(1)
+    tiny = (torch.rand(2, 2 * width, generator=g) + 0.5) * (3e-20 if act == "swiglu" else 6e-39)
+    deep = torch.rand(2, 2 * width, generator=g) + 0.5
+    deep[:, :width] = -88.0 + torch.rand(2, width, generator=g)
+    if act == "gelu":
+        deep = -(torch.rand(2, 2 * width, generator=g) * 0.15 + 9.85)    # sigmoid(2u) down to e^-87 at -10
+    x = torch.cat([tiny, deep]).to(torch.bfloat16)
+    q, s = backend.quantize_rows_int8(x.to(cuda), activation=act)
+    v = _act64(x, act)
+    top = v.abs().amax(1, keepdim=True)
+    # the argument of exp is about 88 here, and off by up to four roundings: 88 * 4 * 2^-24 < 2^-15
+    rel = 2.0 ** -15
+    assert torch.allclose(s.cpu().double(), top[:, 0] / 127, rtol=rel + 2.0 ** -23, atol=2.0 ** -149)
+    assert float((q.cpu().double() - v * 127 / top).abs().max()) <= 0.5 + 127 * 2 * rel
+
+
 def test_rows_with_a_pitch_an_offset_and_three_dimensions(cuda):
     from fp8_gmm_b200 import backend
 
