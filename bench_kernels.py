@@ -1,4 +1,4 @@
-"""Per-kernel microbenchmarks (CUDA-event timed) for the three kernel families of fp8_gmm_b200.
+"""Per-kernel microbenchmarks (CUDA-event timed) for the kernel families of fp8_gmm_b200.
 
     python bench_kernels.py gemm  [--groups G --rows R --n N --k K --act none|gelu|swiglu --a-format e4m3|e5m2]
     python bench_kernels.py wgrad [--groups G --rows R --n N --k K]
@@ -8,6 +8,8 @@
     python bench_kernels.py pad   [--groups G --max-rows M --cols K --mode cast|amax+cast|transpose|quantize|dswiglu|dswiglu+transpose]
                                                   # default = the pad-fusion microbenchmark: 256 groups, rows ~ U[0,4096],
                                                   # K = 7168, bf16 ~ N(0,3) with 0.1 % outliers x100
+    python bench_kernels.py int8  [--groups G --rows R --n N --k K --act none|gelu|swiglu]   # row quantisation, product, both
+    python bench_kernels.py clip  [--rows R --cols K]   # gradient norm and clipping of one R x K bf16 gradient into fp32
     common: [--iters I --warmup W]
 
 Every sub-command prints one JSON line.  GEMMs report TFLOP/s (algorithmic FLOPs, true rows) and the
@@ -285,9 +287,41 @@ def pad_suite(backend, dev, groups=256, max_rows=4096, cols=7168, iters=5, warmu
     return out
 
 
+def int8_case(backend, dev, sizes, n, k, act, iters, warmup):
+    """The int8 experts: rows quantised (behind ``act``), the grouped product, and both in one call."""
+    G, m = len(sizes), sum(sizes)
+    act = None if act == "none" else act
+    x = torch.randn(m, 2 * k if act == "swiglu" else k, dtype=torch.bfloat16, device=dev)
+    w = torch.randint(-127, 128, (G, n, k), dtype=torch.int8, device=dev)
+    ws = torch.rand(G, n, device=dev) / 1000
+    q, s = backend.quantize_rows_int8(x, activation=act)
+    c = torch.empty(m, n, dtype=torch.bfloat16, device=dev)
+    times = [time_ms(fn, iters, warmup) for fn in (lambda: backend.quantize_rows_int8(x, activation=act, codes=q, scales=s),
+                                                   lambda: backend.int8_gmm(q, w, sizes, s, ws, c=c),
+                                                   lambda: backend.int8_linear(x, w, sizes, ws, activation=act, c=c))]
+    backend.device_status()
+    hbm, bf16, src = peaks()
+    row_bytes, tops = 2 * x.numel() + m * k, 2.0 * m * n * k / times[1] / 1e9
+    return {"kernel": "int8", "clocks": LAST_CLOCKS, "groups": G, "rows": m, "n": n, "k": k, "act": act, "quantise_ms": times[0],
+            "quantise_GBps": row_bytes / times[0] / 1e6, "product_ms": times[1], "product_tops": tops, "frac_of_2x_bf16_" + src: tops / (2 * bf16),
+            "weights_GBps": G * n * k / times[1] / 1e6, "both_ms": times[2]}
+
+
+def clip_case(backend, dev, rows, cols, iters, warmup):
+    """Norm, and norm + clipping into fp32, of one bf16 gradient (2 bytes read; 2 more read and 4 written)."""
+    g = torch.randn(rows, cols, dtype=torch.bfloat16, device=dev)
+    out = torch.empty(rows, cols, device=dev)
+    norm = time_ms(lambda: backend.multi_grad_norm([g]), iters, warmup)
+    clip = time_ms(lambda: backend.multi_clip_grad_norm([g], 1.0, outputs=[out]), iters, warmup)
+    hbm, bf16, src = peaks()
+    gbs = 8 * g.numel() / clip / 1e6
+    return {"kernel": "clip", "clocks": LAST_CLOCKS, "elements": g.numel(), "norm_ms": norm, "norm_GBps": 2 * g.numel() / norm / 1e6, "clip_ms": clip,
+            "clip_GBps": gbs, "frac_of_hbm_" + src: gbs / hbm}
+
+
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("what", choices=["gemm", "wgrad", "step-gemms", "pad", "scaled-mm", "library-step"])
+    p.add_argument("what", choices=["gemm", "wgrad", "step-gemms", "pad", "scaled-mm", "library-step", "int8", "clip"])
     p.add_argument("--groups", type=int, default=None)
     p.add_argument("--rows", type=int, default=32768)
     p.add_argument("--n", type=int, default=4096)
@@ -315,6 +349,10 @@ def main():
     elif args.what == "scaled-mm":
         sizes = even_sizes(args.groups or 8, args.rows)
         print(json.dumps(scaled_mm_case(dev, sizes, args.n, args.k, args.iters, args.warmup, "custom")))
+    elif args.what == "int8":
+        print(json.dumps(int8_case(backend, dev, even_sizes(args.groups or 8, args.rows), args.n, args.k, args.act, args.iters, args.warmup)))
+    elif args.what == "clip":
+        print(json.dumps(clip_case(backend, dev, args.rows, args.cols, args.iters, args.warmup)))
     elif args.what == "library-step":
         print(json.dumps(library_gemm_suite(backend, dev, even_sizes(8, 32768), args.iters, args.warmup)))
     elif args.what == "wgrad":

@@ -1,7 +1,8 @@
 """GPU: global gradient norm and clipping against 64 bits.
 
-The squares are summed in (or into) double precision, so the norm is off by its own rounding to fp32 and at most as much
-again from fp32 partial sums: 2^-23 relative.  A clipped element is g * coef with coef rounded to fp32 (2^-24) and the
+Eight squares at a time are summed in fp32 by fused multiply-adds, the rest in double: step k rounds a sum of k squares, so if all
+steps err the same way on equal elements eight squares are off by (1 + ... + 8) / 8 = 4.5 halves of a unit, 4.5 * 2^-24 relative,
+the norm by half of that, and its own rounding to fp32 adds 2^-24: 3.25 * 2^-24 < 2^-22.  A clipped element is g * coef with coef rounded to fp32 (2^-24) and the
 product rounded to fp32 (2^-24) and to the output's type (half a step)."""
 import math
 
@@ -38,7 +39,7 @@ def test_norm_and_clip_in_place(cuda, dtypes):
     before = [g.clone() for g in grads]
     want = _norm64(grads)
     norm = backend.multi_grad_norm(grads)
-    assert norm.dtype == F32 and norm.dim() == 0 and abs(float(norm) - want) <= want * 2.0 ** -23
+    assert norm.dtype == F32 and norm.dim() == 0 and abs(float(norm) - want) <= want * 2.0 ** -22
     got = backend.multi_clip_grad_norm(grads, 1.5)
     assert torch.equal(got, norm)
     _check(grads, before, 1.5 / (want + 1e-6))
@@ -57,7 +58,7 @@ def test_clip_into_other_types(cuda, in_types, out_type):
     outs = [torch.full(g.shape, float("nan"), dtype=out_type, device=cuda) for g in grads]
     want = _norm64(grads)
     norm = backend.multi_clip_grad_norm(grads, 0.25, outputs=outs)
-    assert abs(float(norm) - want) <= want * 2.0 ** -23
+    assert abs(float(norm) - want) <= want * 2.0 ** -22
     _check(outs, grads, 0.25 / (want + 1e-6))
     assert all(torch.equal(a, b) for a, b in zip(grads, before))
     # below the limit the values pass unchanged (one rounding to the output's type)
@@ -88,7 +89,7 @@ def test_two_steps_with_the_sum_in_between(cuda):
     grads = _grads(SHAPES, (BF, F32), 3, cuda)
     a = [g.clone() for g in grads]
     squares = backend.multi_sum_squares(grads)
-    assert squares.dtype == torch.float64 and abs(float(squares) - _norm64(grads) ** 2) <= float(squares) * 2.0 ** -22
+    assert squares.dtype == torch.float64 and abs(float(squares) - _norm64(grads) ** 2) <= float(squares) * 2.0 ** -21
     norm = backend.multi_clip(grads, squares, 2.0)
     assert torch.equal(norm, backend.multi_clip_grad_norm(a, 2.0)) and all(torch.equal(x, y) for x, y in zip(grads, a))
     before = [g.clone() for g in grads]
@@ -108,9 +109,9 @@ def test_squares_outside_fp32(cuda, value, dtype):
     if want > torch.finfo(F32).max:
         assert got == float("inf")
         squares = float(backend.multi_sum_squares(grads))
-        assert abs(math.sqrt(squares) - want) <= want * 2.0 ** -23
+        assert abs(math.sqrt(squares) - want) <= want * 2.0 ** -22
     else:
-        assert abs(got - want) <= want * 2.0 ** -23 + 2.0 ** -150
+        assert abs(got - want) <= want * 2.0 ** -22 + 2.0 ** -150
 
 
 def test_mixed_magnitudes_lose_nothing(cuda):
@@ -118,11 +119,11 @@ def test_mixed_magnitudes_lose_nothing(cuda):
     from fp8_gmm_b200 import backend
 
     g = torch.full((300000,), 1e-21, device=cuda)
-    assert abs(float(backend.multi_grad_norm([g])) - _norm64([g])) <= _norm64([g]) * 2.0 ** -23
+    assert abs(float(backend.multi_grad_norm([g])) - _norm64([g])) <= _norm64([g]) * 2.0 ** -22
     g[12345] = 1e-18
-    assert abs(float(backend.multi_grad_norm([g])) - _norm64([g])) <= _norm64([g]) * 2.0 ** -23
+    assert abs(float(backend.multi_grad_norm([g])) - _norm64([g])) <= _norm64([g]) * 2.0 ** -22
     g[12345] = 1e20
-    assert abs(float(backend.multi_grad_norm([g])) - 1e20) <= 1e20 * 2.0 ** -23
+    assert abs(float(backend.multi_grad_norm([g])) - 1e20) <= 1e20 * 2.0 ** -22
 
 
 def test_zero_infinite_and_nan_gradients(cuda):
@@ -167,7 +168,7 @@ def test_views_alignments_and_layouts(cuda):
         before = [g.clone() for g in grads]
         want = _norm64(grads)
         norm = backend.multi_clip_grad_norm(grads, 3.0)
-        assert abs(float(norm) - want) <= want * 2.0 ** -23
+        assert abs(float(norm) - want) <= want * 2.0 ** -22
         _check(grads, before, 3.0 / (want + 1e-6))
         for i in (0, 8200, 8204, 30000, 30001, 30002, 39999):
             assert buf[i] == keep[i]
@@ -183,7 +184,7 @@ def test_more_tensors_than_one_launch_takes(cuda):
     before = [g.clone() for g in grads]
     want = _norm64(grads)
     norm = backend.multi_clip_grad_norm(grads, 1.0)
-    assert abs(float(norm) - want) <= want * 2.0 ** -23
+    assert abs(float(norm) - want) <= want * 2.0 ** -22
     _check(grads, before, 1.0 / (want + 1e-6))
     assert float(backend.multi_grad_norm([])) == 0.0 and float(backend.multi_clip_grad_norm([], 1.0)) == 0.0
     assert float(backend.multi_grad_norm([torch.zeros(0, device=cuda)])) == 0.0
@@ -294,7 +295,7 @@ def test_train_clip_and_evaluate_in_int8(cuda):
         grads = [p.grad.clone() for p in params]
         want = _norm64(grads)
         norm = fg.clip_grad_norm_(params, 1.0)
-        assert abs(float(norm) - want) <= want * 2.0 ** -23 and want > 1.0
+        assert abs(float(norm) - want) <= want * 2.0 ** -22 and want > 1.0
         _check([p.grad for p in params], grads, 1.0 / (want + 1e-6))
         opt.step()
         opt.zero_grad()
