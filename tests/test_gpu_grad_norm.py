@@ -191,6 +191,20 @@ def test_more_tensors_than_one_launch_takes(cuda):
     assert float(backend.multi_clip_grad_norm([torch.zeros(0, device=cuda)], 1.0)) == 0.0
 
 
+def test_more_than_two_to_the_31_elements(cuda):
+    from fp8_gmm_b200 import backend
+
+    n = 2 ** 31 + 12345
+    g = torch.zeros(n, dtype=BF, device=cuda)
+    at = torch.tensor([0, 1, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 1, n - 1], device=cuda)
+    g[at] = torch.tensor([3.0, -1.0, 2.0, 5.0, -7.0, 1.0, 4.0], dtype=BF, device=cuda)
+    before = g[at].clone()
+    want = math.sqrt(105.0)
+    assert abs(float(backend.multi_clip_grad_norm([g], 1.0)) - want) <= want * 2.0 ** -22
+    _check([g[at]], [before], 1.0 / (want + 1e-6))
+    assert int(torch.count_nonzero(g)) == 7
+
+
 def test_refusals(cuda):
     from fp8_gmm_b200 import backend
 

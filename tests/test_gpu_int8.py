@@ -237,6 +237,33 @@ def test_many_rows_in_few_and_many_groups(cuda):
         assert torch.equal(got, _product(a, b, sizes, sa, sb))
 
 
+def test_offsets_beyond_32_bits(cuda):
+    """Codes, results and weights of more than 2^32 bytes: rows and channels at both ends and around the borders."""
+    from fp8_gmm_b200 import backend
+
+    G, n, k, rows = 5, 16384, 65536, 66000          # weights 5.4 GB, codes 4.3 GB, results 2.2 GB
+    g = torch.Generator(device=cuda).manual_seed(1)
+    w = torch.empty(G, n, k, dtype=torch.int8, device=cuda)
+    w.view(torch.int64).random_(generator=g)
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    ws = _scales((G, n), 4).to(cuda)
+    sizes = [65000, 0, 300, 1, 699]
+    codes, scales = backend.quantize_rows_int8(x)
+    pick = torch.tensor([0, 1, 32767, 32768, 64999, 65000, 65299, 65300, 65301, 65536, 65537, 65999], device=cuda)
+    want_q, want_s = _quantize64(x[pick].cpu())
+    assert torch.equal(codes[pick].cpu(), want_q) and torch.equal(scales[pick].cpu(), want_s)
+    del x
+    out = backend.int8_gmm(codes, w, sizes, scales, ws)
+    backend.device_status()
+    ends = torch.tensor(sizes).cumsum(0)
+    for r in pick.tolist():
+        grp = int((ends <= r).sum())
+        cols = torch.tensor([0, 1, n // 2, n - 1], device=cuda)
+        acc = codes[r].double() @ w[grp, cols].double().t()
+        want = (acc.float() * (scales[r] * ws[grp, cols])).to(torch.bfloat16)
+        assert torch.equal(out[r, cols], want), r
+
+
 def test_sizes_on_the_gpu_leave_the_rows_behind_alone(cuda):
     from fp8_gmm_b200 import _lib, backend
 
@@ -378,6 +405,47 @@ def test_captured_experts_follow_new_tokens_routes_and_weights(cuda):
             want = _moe(experts, gate, tokens, E, top_k)
             assert all(torch.equal(o, want) for o in outs)
     fg.backend.device_status()
+
+
+def test_beside_the_fp8_product_on_another_stream(cuda):
+    """Both persistent products own tensor memory and most of an SM's shared memory: launched at the same time they take turns."""
+    from fp8_gmm_b200 import backend
+
+    sizes, n, k = [300, 0, 77, 900], 512, 1024
+    rows = sum(sizes)
+    x = randn_bf16((rows, k), 1).to(cuda)
+    w16 = randn_bf16((4, n, k), 2).to(cuda)
+    w8, ws = backend.quantize_rows_int8(w16)
+    f8 = [t.to(torch.float8_e4m3fn) for t in (x, w16)]
+    one = torch.ones(4, device=cuda)
+    torch.cuda.synchronize()
+    want = backend.int8_linear(x, w8, sizes, ws), backend.fp8_gmm(f8[0], f8[1], sizes, (one, 1), (one, 1))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(backend.int8_linear(x, w8, sizes, ws))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(backend.fp8_gmm(f8[0], f8[1], sizes, (one, 1), (one, 1)))
+    torch.cuda.synchronize()
+    backend.device_status()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_fewer_sms(cuda):
+    """The product keeps to the SMs that the persistent GEMMs may use."""
+    from fp8_gmm_b200 import backend
+
+    w, ws = _codes((3, 1424, 512), 2).to(cuda), _scales((3, 1424), 3).to(cuda)
+    x = randn_bf16((500, 512), 1).to(cuda)
+    want = backend.int8_linear(x, w, [200, 0, 300], ws)
+    try:
+        for sms in (1, 2, 7, 100):
+            backend.set_gemm_sm_limit(sms)
+            assert torch.equal(backend.int8_linear(x, w, [200, 0, 300], ws), want)
+            backend.device_status()
+    finally:
+        backend.set_gemm_sm_limit(0)
 
 
 def test_calls_on_two_streams_at_once(cuda):
