@@ -10,7 +10,6 @@ functions are the allocation-free fast forms the modules use: one base tensor pl
 instead of Python lists of per-group views.
 """
 import array
-import contextlib
 import ctypes
 import math
 import operator
@@ -634,14 +633,13 @@ def grouped_wgrad_rowmajor(dy, x, row_offsets, a_scale_invs, b_scale_invs, c=Non
 # reference, which has FP8 only)
 # ------------------------------------------------------------------------------------------------
 # The calls below can be as short as a few microseconds on the GPU, so their checks build no message unless they fail.
-_NOTHING = contextlib.nullcontext()
-
-
-def _on(device):
-    """Context in which ``device`` is the current one: the launches below go to the stream of their tensors' device."""
+def _enqueue(device, name, fn, *args):
+    """``fn(*args, stream)`` on the current stream of ``device``, the tensors' device, whichever the current device is."""
     if _raw_device is not None and _raw_device() == device.index:
-        return _NOTHING
-    return torch.cuda.device(device)
+        check(fn(*args, _raw_stream(device.index)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream()), name)
 
 
 def _fail(msg):
@@ -715,8 +713,7 @@ def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, sc
     elif not (scales.device == x.device and scales.dtype == torch.float32 and tuple(scales.shape) == lead and scales.is_contiguous()):
         _fail("quantize_rows_int8: bad scales output")
     args.codes, args.scales = codes.data_ptr(), scales.data_ptr()
-    with _on(x.device):
-        check(lib.fp8gmm_quantize_rows_int8(ctypes.byref(args), _stream()), "quantize_rows_int8")
+    _enqueue(x.device, "quantize_rows_int8", lib.fp8gmm_quantize_rows_int8, ctypes.byref(args))
     return codes, scales
 
 
@@ -766,8 +763,7 @@ def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
     _no_grad_wanted("int8_gmm", a_scales)
     args, c, keep = _int8_gemm_args(a.device, rows, k, b, group_sizes, b_scales, c, "int8_gmm")
     args.a, args.a_scales = a.data_ptr(), a_scales.data_ptr()
-    with _on(a.device):
-        check(lib.fp8gmm_int8_grouped_gemm(ctypes.byref(args), _stream()), "int8_gmm")
+    _enqueue(a.device, "int8_gmm", lib.fp8gmm_int8_grouped_gemm, ctypes.byref(args))
     del keep
     return c
 
@@ -785,10 +781,9 @@ def int8_linear(x, weight, group_sizes, weight_scales, indices=None, top_k=1, ac
     g, c, keep = _int8_gemm_args(x.device, rows, k, weight, group_sizes, weight_scales, c, "int8_linear")
     # codes, then scales (K is a multiple of 16), taken per call: graphs captured one after the other would share a buffer that is kept
     scratch = torch.empty(rows * (k + 4), dtype=torch.int8, device=x.device)
-    q.codes = g.a = scratch.data_ptr()
-    q.scales = g.a_scales = scratch.data_ptr() + rows * k
-    with _on(x.device):
-        check(lib.fp8gmm_int8_linear(ctypes.byref(q), ctypes.byref(g), _stream()), "int8_linear")
+    q.codes = g.a = ptr = scratch.data_ptr()
+    q.scales = g.a_scales = ptr + rows * k
+    _enqueue(x.device, "int8_linear", lib.fp8gmm_int8_linear, ctypes.byref(q), ctypes.byref(g))
     del keep
     return c
 
@@ -877,10 +872,9 @@ def multi_sum_squares(grads):
     if not grads:
         return out.zero_()
     descs, device = _grad_descs(grads, None, "multi_sum_squares")
-    with _on(device):
-        ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_sum_squares(descs.buffer_info()[0], len(grads), ws.data_ptr(), ws.numel() * 8, out.data_ptr(), None, _stream()),
-              "multi_sum_squares")
+    ws = _grad_workspace(len(grads), device)
+    _enqueue(device, "multi_sum_squares", lib.fp8gmm_multi_sum_squares, descs.buffer_info()[0], len(grads), ws.data_ptr(), ws.numel() * 8,
+             out.data_ptr(), None)
     return out
 
 
@@ -891,10 +885,9 @@ def multi_grad_norm(grads):
     if not grads:
         return out.zero_()
     descs, device = _grad_descs(grads, None, "multi_grad_norm")
-    with _on(device):
-        ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_sum_squares(descs.buffer_info()[0], len(grads), ws.data_ptr(), ws.numel() * 8, None, out.data_ptr(), _stream()),
-              "multi_grad_norm")
+    ws = _grad_workspace(len(grads), device)
+    _enqueue(device, "multi_grad_norm", lib.fp8gmm_multi_sum_squares, descs.buffer_info()[0], len(grads), ws.data_ptr(), ws.numel() * 8,
+             None, out.data_ptr())
     return out
 
 
@@ -915,8 +908,7 @@ def multi_clip(grads, sum_squares, max_norm, outputs=None):
     norm = torch.empty((), dtype=torch.float32, device=sum_squares.device)
     descs, device = _grad_descs(grads, outputs, "multi_clip") if grads else (array.array("q"), sum_squares.device)
     _require(device == sum_squares.device, "multi_clip: sum_squares is on another device than the gradients")
-    with _on(device):
-        check(lib.fp8gmm_multi_clip(descs.buffer_info()[0], len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr(), _stream()), "multi_clip")
+    _enqueue(device, "multi_clip", lib.fp8gmm_multi_clip, descs.buffer_info()[0], len(grads), sum_squares.data_ptr(), max_norm, norm.data_ptr())
     return norm
 
 
@@ -929,10 +921,9 @@ def multi_clip_grad_norm(grads, max_norm, outputs=None):
     if not grads:
         return norm.zero_()
     descs, device = _grad_descs(grads, outputs, "multi_clip_grad_norm")
-    with _on(device):
-        ws = _grad_workspace(len(grads), device)
-        check(lib.fp8gmm_multi_clip_grad_norm(descs.buffer_info()[0], len(grads), max_norm, ws.data_ptr(), ws.numel() * 8, norm.data_ptr(), _stream()),
-              "multi_clip_grad_norm")
+    ws = _grad_workspace(len(grads), device)
+    _enqueue(device, "multi_clip_grad_norm", lib.fp8gmm_multi_clip_grad_norm, descs.buffer_info()[0], len(grads), max_norm, ws.data_ptr(),
+             ws.numel() * 8, norm.data_ptr())
     return norm
 
 

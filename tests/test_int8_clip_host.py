@@ -142,6 +142,35 @@ def test_python_entries_refuse_cpu_tensors_and_wanted_gradients():
         backend._no_grad_wanted("int8_linear", x)
 
 
+def test_launches_go_to_the_device_of_the_tensors(monkeypatch):
+    """With another device current, the call runs inside torch.cuda.device(the tensors' device) and takes that device's stream."""
+    from fp8_gmm_b200 import backend
+
+    seen = []
+
+    class Device:
+        def __init__(self, device):
+            seen.append(("enter", device.index))
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *exc):
+            seen.append("exit")
+
+    monkeypatch.setattr(backend, "_raw_device", lambda: 0)
+    monkeypatch.setattr(backend, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setattr(backend, "_stream", lambda: 777)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    backend._enqueue(torch.device("cuda", 0), "a", lambda *args: seen.append(args) or 0, 1, 2)
+    assert seen == [(1, 2, 100)]
+    seen.clear()
+    backend._enqueue(torch.device("cuda", 1), "b", lambda *args: seen.append(args) or 0, 3)
+    assert seen == [("enter", 1), (3, 777), "exit"]
+    with pytest.raises(RuntimeError, match="status 1"):
+        backend._enqueue(torch.device("cuda", 1), "c", lambda *args: 1)
+
+
 def test_dense_layouts():
     from fp8_gmm_b200 import backend
 
