@@ -13,7 +13,12 @@
 //     weights and half of the tile's rows, 256 contraction bytes per stage, into a ring of 4 or 3 stages.  Where such tiles would
 //     keep less than half of the GPU loading weights (few experts, few channels, few rows), a tile is 128 channels: the MMA stays
 //     256 wide and its other rows, whatever lies in shared memory behind the weights, are not looked at.
-//   * Accumulators are double-buffered in TMEM; results are transposed through shared memory and written as 256-byte runs.
+//   * Accumulators are double-buffered in TMEM.  A chunk of 32 rows is read as 16 x 8 fragments, transposed by stmatrix into a
+//     box in shared memory and written as 256-byte runs; two groups of four warps take the chunks in turns.  This bounds products
+//     with short contractions (8 x 4096 rows, 28672 channels, 512 contraction bytes, 1.9 GB written: 560 us; with one group that
+//     stored 2 bytes per lane into the box 1123, with two 787, with fragments and stmatrix 690, with the arrival that does not
+//     wait for the stores 599, with the rows' addresses carried along 560; HBM's floor is 308).  With 4096 contraction bytes it
+//     is hidden behind the MMAs.
 // Group sizes come from the host (parameter block) or are read on the device; either way every CTA builds the prefix sums of
 // rows and tiles in shared memory.  Waits on mbarriers are bounded as in gemm_sm100.cu.
 #include <atomic>
@@ -27,7 +32,7 @@ namespace {
 
 constexpr int kMaxGroups = 512;
 constexpr int kStatusBadSizes = 0x400;   // group sizes that are negative or reach behind the last row
-constexpr int kThreads = 192;            // TMA producer warp, MMA warp, four epilogue warps
+constexpr int kThreads = 320;            // TMA producer warp, MMA warp, two groups of four epilogue warps
 constexpr int kChannels = 128;           // channels of one CTA's half of the MMA
 constexpr int kAtomK = 128;              // bytes of contraction in one box: a 128-byte swizzle atom
 constexpr int kAtoms = 2;                // boxes along the contraction per stage
@@ -66,9 +71,30 @@ __device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ uint16_t result_bf16(uint32_t acc, float scale) {
-  const __nv_bfloat16 v = __float2bfloat16_rn(__fmul_rn(__int2float_rn(static_cast<int>(acc)), scale));
-  return *reinterpret_cast<const uint16_t*>(&v);
+// 16 lanes x 32 columns of a warp's quarter of TMEM as four 16 x 8 fragments: registers 4n, 4n + 1 hold lane i / 4, columns
+// 8n + 2 (i % 4) and the next; 4n + 2, 4n + 3 the same of lane 8 + i / 4.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Stores four 8 x 8 matrices of 16-bit elements transposed: lane 8m + i gives the address of matrix m's column i.
+__device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t m0, uint32_t m1, uint32_t m2, uint32_t m3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(m0), "r"(m1), "r"(m2), "r"(m3) : "memory");
+}
+
+// Arrival behind tc_fence_before, which orders the reads of tensor memory against it.  Nothing else has to be visible to the
+// MMA warp; the release of mbar_arrive_cluster would wait for the warp's stores to C.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ float result(uint32_t acc, float row_scale, float channel_scale) {
+  return __fmul_rn(__int2float_rn(static_cast<int>(acc)), __fmul_rn(row_scale, channel_scale));
 }
 
 // Prefix sums of rows and tiles over the groups, by one warp.  Sizes read on the device are cut off at the last row.
@@ -143,7 +169,8 @@ constexpr int kMaxRows = 256;                 // rows of the larger tile
 constexpr int kMaxStages = 12 / kAtoms;
 constexpr int kRingBytes = 6 * 32 * 1024;
 constexpr int kTmemCols = 512;
-constexpr int kBoxBytes = 32 * kChannels * 2; // 32 rows x 128 channels of bf16
+constexpr int kBoxPitch = kChannels * 2 + 16; // bytes: the 16-byte pieces of eight rows lie in different banks
+constexpr int kBoxBytes = 32 * kBoxPitch;     // 32 rows x 128 channels of bf16
 constexpr int kStagingBytes = 2 * kBoxBytes;
 constexpr int kScaleBytes = 2 * kMaxRows * 4;
 constexpr int kTableBytes = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
@@ -159,7 +186,8 @@ __device__ __forceinline__ bool elect_one() {
 // Columns of a tile's MMAs; half of its rows come from each CTA.
 __device__ __forceinline__ int mma_width(int rows) { return (rows + 31) & ~31; }
 
-__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Barrier of one group of epilogue warps.
+__device__ __forceinline__ void epilogue_barrier(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_constant__ Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -190,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), 8);
+      mbar_init(tempty_bar(a), 16);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -303,60 +331,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
     }
     __syncwarp();
   } else {
-    // ===================== epilogue: 128 threads, one channel each =====================
-    // A warp that gave up on a wait goes on through the barriers, which count all four.
-    const int quad = warp & 3, thread = threadIdx.x - 64;
+    // ===================== epilogue: two groups of four warps, 32 channels each, 32 rows at a time in turns =====================
+    // A warp that gave up on a wait goes on through its group's barriers, which count all four.
+    const int quad = warp & 3, group = (warp - 2) >> 2, thread = (threadIdx.x - 64) & 127;
+    const int my_row = ((thread >> 5) * 2 + group) * 32 + lane;   // the row of a tile whose scale this thread fetches
+    const uint8_t* box = staging + group * kBoxBytes;
+    // where this lane's pieces of the transposed fragments go: row lane % 8 of eight, channels 8 (lane / 8) of the warp's 32
+    const uint32_t box_out = smem_u32(box) + (lane & 7) * kBoxPitch + (quad * 32 + (lane >> 3) * 8) * 2;
+    const uint8_t* box_in = box + (thread >> 4) * kBoxPitch + (thread & 15) * 16;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     grid_dependency_wait();
+    Tile next;
+    float next_sa = 0.f, next_sb[4] = {0.f, 0.f, 0.f, 0.f};   // of the row my_row, of channels lane / 4 + 8 j of the warp's
+    // the scales of a tile are fetched while the one before it is written
+    auto fetch = [&](int tile) {
+      if (tile >= total_tiles) return;
+      next = decode_tile(p, row_start, tile_start, tile);
+      const int n0 = next.n0 + rank * p.channels, channel = n0 + quad * 32 + (lane >> 2), n_end = min(n0 + p.channels, p.n);
+      const float* sb = p.b_scales + static_cast<int64_t>(next.group) * p.n + channel;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) next_sb[j] = channel + 8 * j < n_end ? sb[8 * j] : 0.f;
+      if (my_row < next.rows) next_sa = p.a_scales[next.row0 + my_row];
+    };
+    fetch(worker);
     for (int tile = worker; tile < total_tiles; tile += num_workers) {
-      const Tile t = decode_tile(p, row_start, tile_start, tile);
-      const int n0 = t.n0 + rank * p.channels;
-      const int n_end = min(n0 + p.channels, p.n);
-      const int channel = n0 + quad * 32 + lane;
-      const float sb = channel < n_end ? p.b_scales[static_cast<int64_t>(t.group) * p.n + channel] : 0.f;
+      const Tile t = next;
+      const float sb[4] = {next_sb[0], next_sb[1], next_sb[2], next_sb[3]};
+      const int n0 = t.n0 + rank * p.channels, n_end = min(n0 + p.channels, p.n);
       float* scales = scale_buf + acc * kMaxRows;
-      for (int i = thread; i < t.rows; i += 128) scales[i] = p.a_scales[t.row0 + i];
+      scales[my_row] = next_sa;
+      fetch(tile + num_workers);
       if (lane == 0 && ok) ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 0x8, p.wait_ns);
       ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-      epilogue_barrier();
+      epilogue_barrier(group);
       tc_fence_after();
       const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * kMaxRows) + (static_cast<uint32_t>(quad * 32) << 16);
 
-      for (int c0 = 0; c0 < t.rows; c0 += 32) {
-        uint16_t* box = reinterpret_cast<uint16_t*>(staging + ((c0 >> 5) & 1) * kBoxBytes);
+      // 16 threads write the 256 bytes of a row
+      uint16_t* out = p.c + static_cast<int64_t>(t.row0 + group * 32 + (thread >> 4)) * p.n + n0 + (thread & 15) * 8;
+      const bool writes = n0 + (thread & 15) * 8 < n_end;
+      for (int c0 = group * 32; c0 < t.rows; c0 += 64) {
         if (ok) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c0, r);
+          uint32_t lo[16], hi[16];   // lanes 0-15 and 16-31
+          tmem_ld_16x32(taddr + c0, lo);
+          tmem_ld_16x32(taddr + c0 + (16u << 16), hi);
           tc_wait_ld();
-          uint16_t* mine = box + quad * 32 + lane;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 sa = *reinterpret_cast<const float4*>(scales + c0 + j);
-            mine[(j + 0) * kChannels] = result_bf16(r[j + 0], __fmul_rn(sa.x, sb));
-            mine[(j + 1) * kChannels] = result_bf16(r[j + 1], __fmul_rn(sa.y, sb));
-            mine[(j + 2) * kChannels] = result_bf16(r[j + 2], __fmul_rn(sa.z, sb));
-            mine[(j + 3) * kChannels] = result_bf16(r[j + 3], __fmul_rn(sa.w, sb));
+          for (int n = 0; n < 4; ++n) {
+            const float2 sa = *reinterpret_cast<const float2*>(scales + c0 + 8 * n + 2 * (lane & 3));
+            store_transposed(box_out + 8 * n * kBoxPitch,
+                             pack_bf16x2(result(lo[4 * n], sa.x, sb[0]), result(lo[4 * n + 1], sa.y, sb[0])),
+                             pack_bf16x2(result(lo[4 * n + 2], sa.x, sb[1]), result(lo[4 * n + 3], sa.y, sb[1])),
+                             pack_bf16x2(result(hi[4 * n], sa.x, sb[2]), result(hi[4 * n + 1], sa.y, sb[2])),
+                             pack_bf16x2(result(hi[4 * n + 2], sa.x, sb[3]), result(hi[4 * n + 3], sa.y, sb[3])));
           }
         }
-        epilogue_barrier();
-        // 16 threads write the 256 bytes of a row; the box is free again after the next barrier
-        const int chunk = thread & 15;
-        if (ok && n0 + chunk * 8 < n_end) {
+        epilogue_barrier(group);
+        if (ok && writes) {
+          if (c0 + 32 <= t.rows) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = i * 8 + (thread >> 4);
-            if (c0 + row < t.rows)
-              *reinterpret_cast<uint4*>(p.c + static_cast<int64_t>(t.row0 + c0 + row) * p.n + n0 + chunk * 8) =
-                  *reinterpret_cast<const uint4*>(box + row * kChannels + chunk * 8);
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(i) * 8 * p.n) = *reinterpret_cast<const uint4*>(box_in + i * 8 * kBoxPitch);
+          } else {
+            for (int row = thread >> 4, i = 0; c0 + row < t.rows; row += 8, ++i)
+              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(i) * 8 * p.n) = *reinterpret_cast<const uint4*>(box_in + i * 8 * kBoxPitch);
           }
         }
+        out += static_cast<int64_t>(64) * p.n;
+        epilogue_barrier(group);   // the box is read before it is written again
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(tempty_bar(acc), 0));
-      epilogue_barrier();     // the last box is read before the next tile writes into it
+      if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(tempty_bar(acc), 0));
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }

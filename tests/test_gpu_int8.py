@@ -463,3 +463,21 @@ def test_calls_on_two_streams_at_once(cuda):
                 got[i].append(backend.int8_linear(xs[i], w, sizes[i], ws))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+@pytest.mark.parametrize("k", [16, 272, 512])
+def test_many_tiles_per_cta_with_short_contractions(cuda, k):
+    """Ten and more tiles per CTA pair whose products are done before the tile in front of them is written: the accumulators
+    change hands at the pace of the stores.  Every bit, in each of several runs, and rows behind the last group untouched."""
+    from fp8_gmm_b200 import backend
+
+    sizes, n, spare = [1300, 0, 33, 2077, 257, 1], 16 * 1025, 7
+    rows = sum(sizes)
+    a, b = _codes((rows, k), k).to(cuda), _codes((len(sizes), n, k), k + 1).to(cuda)
+    sa, sb = _scales((rows,), k + 2).to(cuda), _scales((len(sizes), n), k + 3).to(cuda)
+    # |sum| <= 512 * 127^2 < 2^23: each partial sum is exact in the double product, and so is its conversion to fp32
+    want = _product(a, b, sizes, sa, sb)
+    for _ in range(3):
+        c = torch.full((rows + spare, n), 3.0, dtype=torch.bfloat16, device=cuda)
+        backend.int8_gmm(a, b, sizes, sa, sb, c=c[:rows])
+        assert torch.equal(c[:rows], want) and bool((c[rows:] == 3.0).all())
