@@ -464,15 +464,28 @@ int allow_shared_memory() {
 
 int pairs() { return gemm_sms() > 1 ? gemm_sms() / 2 : 1; }
 
+// Time of a tile of up to `rows` rows, in that of one of 128: the weights' loads and the MMAs bound it up to there (204 - 250 ns per
+// 128 bytes of contraction, 380 - 440 with 256 rows; 64 rows 0.9 of 128).
+double tile_time(int64_t rows) { return rows <= 64 ? 0.9 : rows <= 128 ? 1.0 : 1.0 + 0.7 * static_cast<double>(rows - 128) / 128; }
+// Time of the pair with the most tiles: `groups` groups of `mean` rows each in tiles of tile_rows.
+double worker_time(int64_t groups, int64_t mean, int64_t tiles_n, int64_t tile_rows) {
+  const int64_t row_tiles = (mean + tile_rows - 1) / tile_rows;
+  const int64_t most = (groups * row_tiles * tiles_n + pairs() - 1) / pairs();
+  const double full = tile_time(mean < tile_rows ? mean : tile_rows), last = tile_time(mean - (row_tiles - 1) * tile_rows);
+  return full + (most - 1) * ((row_tiles - 1) * full + last) / row_tiles;
+}
+
 // Rows and channels of a tile.  256 rows read the weights least often; 128 are for groups of up to 128 rows (one more stage in
-// flight) and where smaller tiles still fit one wave of the grid; 128 channels where tiles of 256 would fill less than half of it
-// and the time goes into loading weights.  The rule goes by the mean rows of a group that can have any, so that sizes on the host
-// and on the device take the same tile.  Measured, product and quantisation, us.  128 / 256 rows: eight experts of 4096 x 4096
-// with 8 rows each 24.9 / 25.8, with 128 rows 35.4 / 37.1, with 256 rows 46.3 / 47.1, with 1024 rows 125 / 115; 64 experts of 1424 x 2048 with
-// 256 rows 88 / 82; one expert of 1024 x 4096 with 1024 rows 13.9 / 20.1, of 4096 x 14336 with 300 rows 30.0 / 44.2.  128 / 256 channels: one
-// row for each of two experts of 4096 x 14336 24.8 / 27.6, of 4096 x 4096 10.7 / 11.4; one expert of 4096 x 14336 with 16 rows 18.8 / 23.5, with 128 rows
-// 25.7 / 27.8, of 1024 x 4096 with 1024 rows 14.7 / 13.9.  (Splitting the contraction of a partial wave's tiles between pairs, with sums
-// handed on through L2, cost about 8 us a tile: dropped.)
+// flight), for tiles that all fit one wave of the grid, and where the pair with the most tiles is done sooner with them.  128
+// channels where tiles of 256 would fill less than half of the grid (a third with more than 128 rows a group) and the time goes
+// into loading weights.  The rule goes by the mean rows of a group that can have any, so that sizes on the host and on the device
+// take the same tile; the results are the same bits with all.  Measured, us, product alone.  128 / 256 rows: three experts of
+// 3520 x 4096 with 300 rows 17.6 / 26.0, eight of 1536 x 4096 with 300 rows 19.0 / 26.5, with 1000 rows 46.4 / 41.6, eight of 8192 x 4096 with 300 rows
+// 89.4 / 92.6, with 2000 rows 458 / 387.  128 / 256 channels, 128 rows: two rows of 4096 x 14336 24.8 / 27.6, one expert of 256 x 1040 with 300
+// rows 7.3 / 7.9, of 768 x 4096 with 200 rows 9.8 / 10.1, three of 1536 x 4096 with 200 rows 11.4 / 10.6.  Over 405 shapes (1 to 8
+// experts, 64 to 2000 rows each, 256 to 8192 channels, 256 to 4096 bytes) the rule takes 0.6 % more than the best tile on average.
+// (Splitting the contraction of a partial wave's tiles between pairs, with sums handed on through L2, cost about 8 us a
+// tile: dropped.)
 struct TileShape {
   int rows, channels;
 };
@@ -481,9 +494,11 @@ TileShape choose_tile(const fp8gmm_int8_gemm_args* a) {
   const int64_t groups = a->rows < a->num_groups ? a->rows : a->num_groups;
   const int64_t mean = (a->rows + groups - 1) / groups;
   const int64_t small = groups * ((mean + 127) / 128) * tiles_n;   // tiles of 128 rows and 256 channels
+  const bool few = mean <= 128 || small <= pairs() || worker_time(groups, mean, tiles_n, 128) < worker_time(groups, mean, tiles_n, 256);
+  const bool narrow = few && (mean <= 128 ? 2 : 3) * small <= pairs();
   TileShape t;
-  t.rows = g_tile_rows != 0 ? g_tile_rows : mean <= 128 || small <= pairs() ? 128 : 256;
-  t.channels = g_channels != 0 ? g_channels / 2 : mean <= 128 && 2 * small <= pairs() ? kChannels / 2 : kChannels;
+  t.rows = g_tile_rows != 0 ? g_tile_rows : few ? 128 : 256;
+  t.channels = g_channels != 0 ? g_channels / 2 : narrow ? kChannels / 2 : kChannels;
   return t;
 }
 
