@@ -79,6 +79,7 @@ class QuantizeRowsArgs(ctypes.Structure):
     _fields_ = [
         ("in_", c_vp), ("in_ld", c_i64), ("indices", c_vp), ("top_k", ctypes.c_int), ("in_rows", c_i64),
         ("rows", c_i64), ("cols", c_i64), ("activation", ctypes.c_int), ("codes", c_vp), ("scales", c_fp),
+        ("codes_ld", c_i64),
     ]
 
 
@@ -86,7 +87,7 @@ class Int8GemmArgs(ctypes.Structure):
     _fields_ = [
         ("a", c_vp), ("b", c_vp), ("c", c_vp), ("a_scales", c_fp), ("b_scales", c_fp),
         ("m_sizes", ctypes.POINTER(c_i64)), ("device_m_sizes", c_vp),
-        ("num_groups", ctypes.c_int), ("rows", c_i64), ("n", c_i64), ("k", c_i64),
+        ("num_groups", ctypes.c_int), ("rows", c_i64), ("n", c_i64), ("k", c_i64), ("a_ld", c_i64),
     ]
 
 

@@ -779,10 +779,13 @@ def int8_linear(x, weight, group_sizes, weight_scales, indices=None, top_k=1, ac
     q, (rows,) = _quantize_args(x, indices, top_k, activation)
     k = q.cols
     g, c, keep = _int8_gemm_args(x.device, rows, k, weight, group_sizes, weight_scales, c, "int8_linear")
-    # codes, then scales (K is a multiple of 16), taken per call: graphs captured one after the other would share a buffer that is kept
-    scratch = torch.empty(rows * (k + 4), dtype=torch.int8, device=x.device)
+    # Codes in rows of whole 128-byte lines (K = 2064 as it is: 115 us against 102 for the product of 8 x 2000 rows and 3520
+    # channels), then scales.  Taken per call: graphs captured one after the other would share a buffer that is kept.
+    pitch = (k + 127) & -128
+    scratch = torch.empty(rows * (pitch + 4), dtype=torch.int8, device=x.device)
     q.codes = g.a = ptr = scratch.data_ptr()
-    q.scales = g.a_scales = ptr + rows * k
+    q.scales = g.a_scales = ptr + rows * pitch
+    q.codes_ld = g.a_ld = pitch
     _enqueue(x.device, "int8_linear", lib.fp8gmm_int8_linear, ctypes.byref(q), ctypes.byref(g))
     del keep
     return c

@@ -237,7 +237,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
   const uint32_t tmem_base = *tmem_base_slot;
   const int worker = blockIdx.x >> 1, num_workers = gridDim.x >> 1;
   const int total_tiles = tile_start[p.num_groups];
-  const int num_kb = (p.k + kBlockK - 1) / kBlockK;
+  // whole stages, then 32-byte steps of a last one that ends with the contraction: no box of zeros, no MMAs on zeros (8 x 2000
+  // rows, 3520 channels: K = 544 44.7 -> 41.4 us; tests for it inside the loops made K = 2048 1 - 4 % slower)
+  const int num_kb = (p.k + kBlockK - 1) / kBlockK, full_kb = p.k / kBlockK;
+  const int last_steps = (p.k - full_kb * kBlockK + 31) / 32, last_atoms = (last_steps + kAtomK / 32 - 1) / (kAtomK / 32);
 
   if (warp == 0) {
     // ===================== TMA producer: both CTAs credit the leader's barriers =====================
@@ -255,35 +258,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
       const int yw = t.group * p.n + t.n0 + rank * p.channels, yx = t.row0 + rank * (width / 2);
       const int box = width <= 32 ? 0 : width <= 64 ? 1 : width <= 128 ? 2 : 3;   // box of 16 << box rows: one CTA's half
       const CUtensorMap* map_x = &p.map_x[box];
-      const int bytes = 2 * kAtoms * (w_bytes + (16 << box) * kAtomK);                    // of both CTAs
+      const int bytes = 2 * (w_bytes + (16 << box) * kAtomK);                             // of one box along K, in both CTAs
       int kb = 0;
       if (tile == worker) {
         // Weights do not depend on the kernel before this one (the quantisation of the rows): a ring full of them goes ahead.
         const int first = min(num_kb, stages);
         for (int i = 0; i < first; ++i) {
-          if (leader && issue) mbar_expect_tx(full_bar(i), bytes);
+          const int atoms = i < full_kb ? kAtoms : last_atoms;
+          if (leader && issue) mbar_expect_tx(full_bar(i), atoms * bytes);
 #pragma unroll
           for (int h = 0; h < kAtoms; ++h)
-            if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes + h * w_bytes, &p.map_w, full0_leader + 8u * i, i * kBlockK + h * kAtomK, yw);
+            if (issue && h < atoms) tma_load_2d_pair(tiles_addr + i * stage_bytes + h * w_bytes, &p.map_w, full0_leader + 8u * i, i * kBlockK + h * kAtomK, yw);
         }
         grid_dependency_wait();
         for (int i = 0; i < first; ++i)
 #pragma unroll
           for (int h = 0; h < kAtoms; ++h)
-            if (issue) tma_load_2d_pair(tiles_addr + i * stage_bytes + kAtoms * w_bytes + h * x_bytes, map_x, full0_leader + 8u * i, i * kBlockK + h * kAtomK, yx);
+            if (issue && (h < last_atoms || i < full_kb)) tma_load_2d_pair(tiles_addr + i * stage_bytes + kAtoms * w_bytes + h * x_bytes, map_x, full0_leader + 8u * i, i * kBlockK + h * kAtomK, yx);
         kb = first;
         stage = first == stages ? 0 : first;
         phase = first == stages ? 1u : 0u;
       }
-      for (; kb < num_kb && ok; ++kb) {
+      for (; kb < full_kb && ok; ++kb) {
         ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x1, p.wait_ns);
         if (ok) {
           const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
-          if (leader && issue) mbar_expect_tx(full_bar(stage), bytes);
+          if (leader && issue) mbar_expect_tx(full_bar(stage), kAtoms * bytes);
 #pragma unroll
           for (int h = 0; h < kAtoms; ++h) {
             if (issue) tma_load_2d_pair(sw + h * w_bytes, &p.map_w, bar, kb * kBlockK + h * kAtomK, yw);
             if (issue) tma_load_2d_pair(sw + kAtoms * w_bytes + h * x_bytes, map_x, bar, kb * kBlockK + h * kAtomK, yx);
+          }
+        }
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (kb < num_kb && ok) {
+        ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x1, p.wait_ns);
+        if (ok) {
+          const uint32_t sw = tiles_addr + stage * stage_bytes, bar = full0_leader + 8u * stage;
+          if (leader && issue) mbar_expect_tx(full_bar(stage), last_atoms * bytes);
+#pragma unroll
+          for (int h = 0; h < kAtoms; ++h) {
+            if (issue && h < last_atoms) tma_load_2d_pair(sw + h * w_bytes, &p.map_w, bar, kb * kBlockK + h * kAtomK, yw);
+            if (issue && h < last_atoms) tma_load_2d_pair(sw + kAtoms * w_bytes + h * x_bytes, map_x, bar, kb * kBlockK + h * kAtomK, yx);
           }
         }
         if (++stage == stages) {
@@ -308,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
         if (!ok) break;
         tc_fence_after();
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kMaxRows);
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = 0; kb < full_kb; ++kb) {
           ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, 0x4, p.wait_ns);
           if (!ok) break;
           const uint64_t dw = desc_w0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
@@ -324,6 +344,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
           }
         }
         if (!ok) break;
+        if (full_kb < num_kb) {
+          ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, 0x4, p.wait_ns);
+          if (!ok) break;
+          const uint64_t dw = desc_w0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
+          const uint64_t dx = desc_x0 + static_cast<uint64_t>(stage * (stage_bytes >> 4));
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k)
+            if (issue && k < last_steps)
+              umma_i8_pair(tmem_d, dw + (k >> 2) * (w_bytes >> 4) + 2 * (k & 3), dx + (k >> 2) * (x_bytes >> 4) + 2 * (k & 3), idesc, (full_kb | k) != 0 ? 1u : 0u);
+          if (issue) umma_commit_pair(empty_bar(stage));
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
         if (issue) umma_commit_pair(tfull_bar(acc));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
@@ -426,15 +461,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-// (rows x cols) bytes, row pitch cols, box of box_rows x 128 bytes, SWIZZLE_128B.
-int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows) {
+// (rows x cols) bytes, row pitch `pitch`, box of box_rows x 128 bytes, SWIZZLE_128B.
+int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows) {
   auto fn = get_encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is not available from this driver");
     return FP8GMM_CUDA_ERROR;
   }
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
   const cuuint32_t box[2] = {kAtomK, static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
@@ -510,6 +545,8 @@ int int8_gemm_check(const fp8gmm_int8_gemm_args* a) {
   FP8GMM_CHECK_ARG(a->num_groups >= 0 && a->num_groups <= kMaxGroups, "int8_grouped_gemm: num_groups %d outside [0, %d]", a->num_groups, kMaxGroups);
   FP8GMM_CHECK_ARG(a->n > 0 && a->k > 0 && a->n % 16 == 0 && a->k % 16 == 0, "int8_grouped_gemm: N (%lld) and K (%lld) must be positive multiples of 16",
                    (long long)a->n, (long long)a->k);
+  FP8GMM_CHECK_ARG(a->a_ld == 0 || (a->a_ld >= a->k && a->a_ld <= INT32_MAX && a->a_ld % 16 == 0),
+                   "int8_grouped_gemm: a row pitch of %lld is not a multiple of 16 from K = %lld to 2^31", (long long)a->a_ld, (long long)a->k);
   FP8GMM_CHECK_ARG(a->k < (1 << 17), "int8_grouped_gemm: K = %lld could overflow the 32-bit sums (K < 131072)", (long long)a->k);
   FP8GMM_CHECK_ARG(a->n <= INT32_MAX / (a->num_groups > 0 ? a->num_groups : 1) - 1024, "int8_grouped_gemm: too many weight rows");
   FP8GMM_CHECK_ARG(a->rows >= 0 && a->rows <= INT32_MAX - 1024, "int8_grouped_gemm: bad number of rows");
@@ -550,10 +587,10 @@ int int8_gemm_launch(const fp8gmm_int8_gemm_args* a, void* stream, bool after_qu
   const TileShape tile = choose_tile(a);
   const int tile_rows = p.tile_rows = tile.rows;
   p.channels = tile.channels;
-  rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, p.channels);
+  rc = encode_rows(&p.map_w, a->b, a->num_groups * a->n, a->k, a->k, p.channels);
   if (rc != FP8GMM_OK) return rc;
   for (; p.x_maps < 4 && (p.x_maps == 0 || (32 << p.x_maps <= tile_rows && 16 << p.x_maps < p.rows)); ++p.x_maps) {
-    rc = encode_rows(&p.map_x[p.x_maps], a->a, a->rows, a->k, 16 << p.x_maps);
+    rc = encode_rows(&p.map_x[p.x_maps], a->a, a->rows, a->k, a->a_ld != 0 ? a->a_ld : a->k, 16 << p.x_maps);
     if (rc != FP8GMM_OK) return rc;
   }
   // with 64 channels the MMA reads 16 KiB from the start of each half of the weights all the same: into what lies behind them
@@ -591,8 +628,8 @@ int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* a, void* stream) { ret
 
 int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gemm_args* g, void* stream) {
   FP8GMM_CHECK_ARG(q != nullptr && g != nullptr, "int8_linear: NULL arguments");
-  FP8GMM_CHECK_ARG(q->codes == g->a && q->scales == g->a_scales && q->rows == g->rows && q->cols == g->k,
-                   "int8_linear: the product has to take the codes, scales, rows and columns of the quantisation");
+  FP8GMM_CHECK_ARG(q->codes == g->a && q->scales == g->a_scales && q->rows == g->rows && q->cols == g->k && q->codes_ld == g->a_ld,
+                   "int8_linear: the product has to take the codes, scales, rows, columns and row pitch of the quantisation");
   int rc = fp8gmm::int8_gemm_check(g);   // before anything is launched
   if (rc != FP8GMM_OK) return rc;
   rc = fp8gmm_quantize_rows_int8(q, stream);

@@ -33,6 +33,7 @@ struct QuantRowsParams {
   int64_t in_rows;
   int64_t rows, cols;  // of the codes
   int8_t* codes;
+  int64_t codes_ld;
   float* scales;
   int* status;
 };
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_A
   if (!live) return;
   if (threadIdx.x == 0) p.scales[r] = s.scale;
   const bool zero = s.pre == 0.f;
-  uint2* out = reinterpret_cast<uint2*>(p.codes + r * p.cols);
+  uint2* out = reinterpret_cast<uint2*>(p.codes + r * p.codes_ld);
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
     const int c = threadIdx.x + u * blockDim.x;
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
     for (int64_t c = threadIdx.x; c < p.cols; c += kLongThreads) {
       uint32_t q = 0;
       if (!zero) q = code_of<kAct>(activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f), s);
-      p.codes[r * p.cols + c] = static_cast<int8_t>(q & 0xFFu);
+      p.codes[r * p.codes_ld + c] = static_cast<int8_t>(q & 0xFFu);
     }
   }
 }
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
 template <int kAct>
 void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
   const int64_t vecs = p.cols / 8;
-  const bool aligned = p.cols % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
+  const bool aligned = p.cols % 8 == 0 && p.codes_ld % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
   if (aligned && vecs <= kMaxThreads * kMaxVecs && p.rows <= INT32_MAX) {
     // Four vectors per thread keep more bytes in flight (measured against two: 32768 rows of 4096 69 / 81 us, behind SwiGLU
     // 14336 wide 384 / 434 us = 6.1 TB/s); two answer sooner where all rows run at once, and fill a warp with a short row
@@ -236,6 +237,8 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) 
                    "quantize_rows_int8: unknown activation %d", a->activation);
   const int64_t width = a->activation == FP8GMM_ACT_SWIGLU ? 2 * a->cols : a->cols;
   FP8GMM_CHECK_ARG(a->in_ld >= width, "quantize_rows_int8: a row pitch of %lld is shorter than a row of %lld", (long long)a->in_ld, (long long)width);
+  FP8GMM_CHECK_ARG(a->codes_ld == 0 || a->codes_ld >= a->cols, "quantize_rows_int8: a row pitch of %lld is shorter than the codes' %lld",
+                   (long long)a->codes_ld, (long long)a->cols);
   if (a->rows == 0) return FP8GMM_OK;   // `indices` may then be a NULL that stands for an empty array
   FP8GMM_CHECK_ARG(a->indices != nullptr ? a->top_k > 0 : a->in_rows == a->rows, "quantize_rows_int8: %s",
                    a->indices != nullptr ? "top_k must be positive" : "row counts differ");
@@ -250,6 +253,7 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* a, void* stream) 
   p.rows = a->rows;
   p.cols = a->cols;
   p.codes = static_cast<int8_t*>(a->codes);
+  p.codes_ld = a->codes_ld != 0 ? a->codes_ld : a->cols;
   p.scales = a->scales;
   p.status = device_status_word();
   FP8GMM_CHECK_ARG(p.status != nullptr, "quantize_rows_int8: cannot resolve the device status word");

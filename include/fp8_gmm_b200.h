@@ -422,8 +422,9 @@ typedef struct {
   int64_t rows;
   int64_t cols;           /* columns of codes */
   int activation;
-  void* codes;            /* int8 (rows x cols) row-major */
+  void* codes;            /* int8 (rows x cols) */
   float* scales;          /* fp32[rows] */
+  int64_t codes_ld;       /* row pitch of codes; 0 = cols */
 } fp8gmm_quantize_rows_args;
 
 int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* args, void* stream);
@@ -431,7 +432,8 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* args, void* strea
 /*
  * C[r, :] = bf16( (sum_k a[r, k] * b[g, :, k]) * a_scales[r] * b_scales[g, :] ) for every row r of group g; 32-bit integer
  * sums (exact: K < 131072).
- *   a        int8 (rows x K) row-major, groups are consecutive row blocks
+ *   a        int8 (rows x K), groups are consecutive row blocks; row pitch a_ld (a multiple of 16, 0 = K; one that is a
+ *            multiple of 128 is read fastest)
  *   b        int8 (G x N x K) row-major
  *   c        bf16 (rows x N)
  *   m_sizes  HOST int64[num_groups], sum = rows; or NULL and
@@ -453,12 +455,13 @@ typedef struct {
   int64_t rows;
   int64_t n;
   int64_t k;
+  int64_t a_ld;
 } fp8gmm_int8_gemm_args;
 
 int fp8gmm_int8_grouped_gemm(const fp8gmm_int8_gemm_args* args, void* stream);
 
 /* Both calls, the second on the codes and scales that the first writes (q->codes == g->a, q->scales == g->a_scales, the same
- * rows and columns); the product starts loading weights while the rows are still being quantised. */
+ * rows, columns and row pitch); the product starts loading weights while the rows are still being quantised. */
 int fp8gmm_int8_linear(const fp8gmm_quantize_rows_args* q, const fp8gmm_int8_gemm_args* g, void* stream);
 
 /* Process-wide switch of the launches above, for tests and experiments: rows and channels of a tile (128 or 256 each; 0 = chosen

@@ -481,3 +481,49 @@ def test_many_tiles_per_cta_with_short_contractions(cuda, k):
         c = torch.full((rows + spare, n), 3.0, dtype=torch.bfloat16, device=cuda)
         backend.int8_gmm(a, b, sizes, sa, sb, c=c[:rows])
         assert torch.equal(c[:rows], want) and bool((c[rows:] == 3.0).all())
+
+
+@pytest.mark.parametrize("pitch,cols", [(128, 96), (144, 144), (96, 80), (75, 75), (81, 48), (16500, 16400)])
+def test_codes_and_operands_with_a_row_pitch(cuda, pitch, cols):
+    """Through the C interface: codes written with a pitch leave the gaps alone, a product reads them with it."""
+    import ctypes
+
+    from fp8_gmm_b200 import _lib, backend
+
+    rows = 37
+    x = randn_bf16((rows, cols), pitch).to(cuda)
+    want_q, want_s = backend.quantize_rows_int8(x)
+    codes = torch.full((rows, pitch), 99, dtype=torch.int8, device=cuda)
+    scales = torch.empty(rows, device=cuda)
+    q = _lib.QuantizeRowsArgs(in_=x.data_ptr(), in_ld=cols, top_k=1, in_rows=rows, rows=rows, cols=cols, activation=0,
+                              codes=codes.data_ptr(), scales=scales.data_ptr(), codes_ld=pitch)
+    _lib.check(_lib.lib.fp8gmm_quantize_rows_int8(ctypes.byref(q), torch.cuda.current_stream().cuda_stream), "quantise")
+    assert torch.equal(codes[:, :cols], want_q) and bool((codes[:, cols:] == 99).all()) and torch.equal(scales, want_s)
+    if pitch % 16 or cols % 16:
+        return
+    sizes, n = [30, 7], 48
+    b, sb = _codes((2, n, cols), 1).to(cuda), _scales((2, n), 2).to(cuda)
+    want = backend.int8_gmm(want_q, b, sizes, want_s, sb)
+    c = torch.zeros(rows, n, dtype=torch.bfloat16, device=cuda)
+    host_sizes = (ctypes.c_int64 * 2)(*sizes)
+    g = _lib.Int8GemmArgs(a=codes.data_ptr(), b=b.data_ptr(), c=c.data_ptr(), a_scales=scales.data_ptr(), b_scales=sb.data_ptr(),
+                          num_groups=2, rows=rows, n=n, k=cols, a_ld=pitch)
+    g.m_sizes = ctypes.cast(host_sizes, ctypes.POINTER(ctypes.c_int64))
+    _lib.check(_lib.lib.fp8gmm_int8_grouped_gemm(ctypes.byref(g), torch.cuda.current_stream().cuda_stream), "product")
+    assert torch.equal(c, want)
+
+
+@pytest.mark.parametrize("k", [16, 48, 112, 144, 240, 272, 400, 528, 1040])
+@pytest.mark.parametrize("channels", [128, 256])
+def test_contractions_that_end_inside_a_stage(cuda, any_variant, k, channels):
+    """Every number of 32-byte steps and boxes in the last stage, wide and narrow tiles; what lies behind a row is the next one,
+    with codes that would show in the sums."""
+    from fp8_gmm_b200 import backend
+
+    sizes, n = [5, 140, 0, 33], 208
+    rows = sum(sizes)
+    a, b = _codes((rows, k), k + 5), _codes((4, n, k), k + 6)
+    sa, sb = _scales((rows,), 7), _scales((4, n), 8)
+    backend.set_int8_variant(128, channels)
+    got = backend.int8_gmm(a.to(cuda), b.to(cuda), sizes, sa.to(cuda), sb.to(cuda))
+    assert torch.equal(got.cpu(), _product(a, b, sizes, sa, sb))

@@ -43,6 +43,7 @@ def _gemm_args(**kw):
     (dict(rows=9), b"sum to 8"), (dict(rows=7), b"bad size"), (dict(rows=-1), b"number of rows"), (dict(num_groups=513), b"num_groups"),
     (dict(num_groups=-1), b"num_groups"), (dict(device_m_sizes=256), b"not both"), (dict(m_sizes=None), b"not both"),
     (dict(a=None), b"NULL"), (dict(b_scales=None), b"NULL"), (dict(b=264), b"aligned"), (dict(n=16 << 27), b"weight rows"),
+    (dict(a_ld=48), b"pitch"), (dict(a_ld=72), b"pitch"), (dict(a_ld=-64), b"pitch"), (dict(a_ld=1 << 31), b"pitch"),
 ])
 def test_int8_gemm_refusals(change, message):
     L = _lib()
@@ -66,6 +67,7 @@ def test_int8_gemm_negative_group_is_refused_and_no_rows_are_fine():
 @pytest.mark.parametrize("change,message", [
     (dict(rows=-1), b"negative"), (dict(activation=3), b"activation"), (dict(in_ld=63), b"pitch"), (dict(activation=2), b"pitch"),
     (dict(in_rows=5), b"row counts"), (dict(indices=256, top_k=0), b"top_k"), (dict(codes=None), b"NULL"), (dict(cols=0, in_ld=0), b"no columns"),
+    (dict(codes_ld=63), b"pitch"), (dict(codes_ld=-64), b"pitch"),
 ])
 def test_quantize_rows_refusals(change, message):
     L = _lib()
