@@ -733,12 +733,18 @@ def _int8_gemm_args(device, rows, k, b, group_sizes, b_scales, c, name):
         _fail(f"{name}: bad output")
     args = Int8GemmArgs()
     keep = None
-    if isinstance(group_sizes, torch.Tensor) and group_sizes.is_cuda:
+    if isinstance(group_sizes, torch.Tensor):
         if group_sizes.shape != (G,):
             _fail(f"{name}: one group size per expert is required")
-        if not (group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.is_contiguous()):
-            _fail(f"{name}: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of the rows")
-        args.device_m_sizes = group_sizes.data_ptr()
+        if group_sizes.is_cuda:
+            if not (group_sizes.device == device and group_sizes.dtype == torch.int64 and group_sizes.is_contiguous()):
+                _fail(f"{name}: group sizes on the GPU must be a contiguous 1-D int64 tensor on the device of the rows")
+            args.device_m_sizes = group_sizes.data_ptr()
+        elif group_sizes.dtype == torch.int64 and group_sizes.is_contiguous() and group_sizes.is_cpu:
+            # as _i64_array, without its two conversions and the cast (0.5 us instead of 2)
+            args.m_sizes, keep = (ctypes.c_int64 * G).from_address(group_sizes.data_ptr()), group_sizes
+        else:
+            args.m_sizes, keep = _i64_array(group_sizes)
     else:
         if len(group_sizes) != G:
             _fail(f"{name}: one group size per expert is required")

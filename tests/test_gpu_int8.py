@@ -527,3 +527,21 @@ def test_contractions_that_end_inside_a_stage(cuda, any_variant, k, channels):
     backend.set_int8_variant(128, channels)
     got = backend.int8_gmm(a.to(cuda), b.to(cuda), sizes, sa.to(cuda), sb.to(cuda))
     assert torch.equal(got.cpu(), _product(a, b, sizes, sa, sb))
+
+
+def test_group_sizes_in_every_form_on_the_host(cuda):
+    """Lists, int32 and strided tensors give what a contiguous int64 tensor gives; other shapes are refused; no groups, no rows."""
+    from fp8_gmm_b200 import backend
+
+    sizes = [3, 0, 9]
+    x = randn_bf16((12, 64), 1).to(cuda)
+    w, ws = backend.quantize_rows_int8(randn_bf16((3, 32, 64), 2).to(cuda))
+    want = backend.int8_linear(x, w, torch.tensor(sizes), ws)
+    strided = torch.tensor([[3, 7], [0, 7], [9, 7]])[:, 0]
+    for form in (sizes, tuple(sizes), torch.tensor(sizes, dtype=torch.int32), strided, torch.tensor(sizes, device=cuda)):
+        assert torch.equal(backend.int8_linear(x, w, form, ws), want)
+    for bad in (torch.tensor([sizes, sizes, sizes]), torch.tensor([12]), torch.tensor(12), [12]):
+        with pytest.raises(RuntimeError, match="group size"):
+            backend.int8_linear(x, w, bad, ws)
+    for none in ([], torch.empty(0, dtype=torch.int64)):
+        assert backend.int8_linear(x[:0], w[:0], none, ws[:0]).shape == (0, 32)
