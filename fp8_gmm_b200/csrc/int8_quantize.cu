@@ -40,24 +40,70 @@ struct QuantRowsParams {
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
 
+// Two floats in a register pair: one instruction for both where there is a packed form, each rounded as on its own.  The kernel is
+// bound by its instructions as much as by HBM: 32768 rows of 4096 took 69 us with single ones and 61.5 with these; behind GELU 89
+// and 77, behind SwiGLU 106 and 102.  (Behind an activation the special function unit is next, two operations an element at an
+// eighth of the rate; one reciprocal shared by two elements saved a quarter of them and cost more in the test for its range: 93.)
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ Pair both(float a) { return pair_of(a, a); }
+__device__ __forceinline__ float2 split(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // a / (1 + 2^p) from the hardware's exp2 and reciprocal, a few ulp (the rounding of exp2's argument, |p| 2^-24, is larger from
 // |p| = 4 on).  Both instructions flush subnormal numbers, so the quotient is taken 16 times as large, 16 / (1 + e) =
 // 1 / (1/16 + 2^(p - 4)): it then stays normal for every e = 2^p in fp32's range.  An exp that overflows gives 0.
+// The two share a reciprocal, 1 / d = d' / (d d'), unless d d' leaves the range in which that stays normal: the special function
+// unit, at an eighth of the others' rate, is what limits this kernel behind an activation.
 constexpr float kLog2E = 1.44269504f;
-__device__ __forceinline__ float over_one_plus_exp2(float a, float power_minus_4) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(power_minus_4));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 0.0625f));
-  return a * 0.0625f * r;
+__device__ __forceinline__ Pair over_one_plus_exp2(Pair a, Pair powers_minus_4) {
+  const float2 p = split(powers_minus_4);
+  const float2 d = split(add2(pair_of(exp2_approx(p.x), exp2_approx(p.y)), both(0.0625f)));
+  const Pair inv = pair_of(rcp_approx(d.x), rcp_approx(d.y));
+  return mul2(mul2(a, both(0.0625f)), inv);
 }
 template <int kAct>
-__device__ __forceinline__ float activated(float a, float b) {
-  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return over_one_plus_exp2(a, fmaf(a, -kLog2E, -4.f)) * b;
+__device__ __forceinline__ Pair activated(Pair a, Pair b) {
+  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return mul2(over_one_plus_exp2(a, fma2(a, both(-kLog2E), both(-4.f))), b);
   if constexpr (kAct == FP8GMM_ACT_GELU) {
     // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), without the cancellation of 1 + tanh u at
     // negative u; the power of two is -2u log2(e) = a (c + 0.044715 c a^2)
     constexpr float kC = -2.f * 0.79788456f * kLog2E;
-    return over_one_plus_exp2(a, fmaf(a, fmaf(a * a, 0.044715f * kC, kC), -4.f));
+    return over_one_plus_exp2(a, fma2(a, fma2(mul2(a, a), both(0.044715f * kC), both(kC)), both(-4.f)));
   }
   return a;
 }
@@ -84,16 +130,20 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
   }
   return s;
 }
-// The code in the low byte: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.  Behind
+// The codes in the low bytes: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.  Behind
 // an activation there are no exact ties to respect (v itself is rounded), and the quotient is not corrected.
 template <int kAct>
-__device__ __forceinline__ uint32_t code_of(float v, const RowScale& s) {
-  constexpr float kMagic = 12582912.f;
-  const float t = v * s.pre;
-  if constexpr (kAct != FP8GMM_ACT_NONE) return __float_as_uint(fmaf(t, s.inv, kMagic));
-  float y = t * s.inv;
-  y = fmaf(fmaf(-y, s.top, t), s.inv, y);
-  return __float_as_uint(y + kMagic);
+__device__ __forceinline__ uint2 codes_of(Pair v, const RowScale& s) {
+  const Pair magic = both(12582912.f), t = mul2(v, both(s.pre));
+  Pair y;
+  if constexpr (kAct != FP8GMM_ACT_NONE) {
+    y = fma2(t, both(s.inv), magic);
+  } else {
+    y = mul2(t, both(s.inv));
+    y = add2(fma2(fma2(y, both(-s.top), t), both(s.inv), y), magic);
+  }
+  const float2 r = split(y);
+  return make_uint2(__float_as_uint(r.x), __float_as_uint(r.y));
 }
 // max(a, |b|), NaN if either is
 __device__ __forceinline__ float max_abs(float a, float b) {
@@ -141,7 +191,7 @@ __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_A
     raw[u] = in ? __ldg(a + c) : make_uint4(0, 0, 0, 0);
     if constexpr (kAct == FP8GMM_ACT_SWIGLU) raw2[u] = in ? __ldg(a + vecs + c) : make_uint4(0, 0, 0, 0);   // [gate | up]
   }
-  float v[kVecs][8];
+  Pair v[kVecs][4];
   float top = 0.f;
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
@@ -150,9 +200,9 @@ __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_A
     if constexpr (kAct == FP8GMM_ACT_SWIGLU) w2[0] = raw2[u].x, w2[1] = raw2[u].y, w2[2] = raw2[u].z, w2[3] = raw2[u].w;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[u][2 * j] = activated<kAct>(bf16_lo(w[j]), bf16_lo(w2[j]));
-      v[u][2 * j + 1] = activated<kAct>(bf16_hi(w[j]), bf16_hi(w2[j]));
-      top = max_abs(max_abs(top, v[u][2 * j]), v[u][2 * j + 1]);
+      v[u][j] = activated<kAct>(pair_of(bf16_lo(w[j]), bf16_hi(w[j])), pair_of(bf16_lo(w2[j]), bf16_hi(w2[j])));
+      const float2 x = split(v[u][j]);
+      top = max_abs(max_abs(top, x.x), x.y);
     }
   }
   const RowScale s = row_scale(row_max(__float_as_uint(top), warp_max + threadIdx.y * (blockDim.x >> 5)));
@@ -167,10 +217,8 @@ __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_A
     uint32_t q[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float* x = &v[u][4 * h];
-      const uint32_t lo = __byte_perm(code_of<kAct>(x[0], s), code_of<kAct>(x[1], s), 0x0040);
-      const uint32_t hi = __byte_perm(code_of<kAct>(x[2], s), code_of<kAct>(x[3], s), 0x0040);
-      q[h] = zero ? 0u : __byte_perm(lo, hi, 0x5410);
+      const uint2 a2 = codes_of<kAct>(v[u][2 * h], s), b2 = codes_of<kAct>(v[u][2 * h + 1], s);
+      q[h] = zero ? 0u : __byte_perm(__byte_perm(a2.x, a2.y, 0x0040), __byte_perm(b2.x, b2.y, 0x0040), 0x5410);
     }
     out[c] = make_uint2(q[0], q[1]);
   }
@@ -185,19 +233,26 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
     const int64_t src = source_row(p, r);
     const uint16_t* a = p.in + (src < 0 ? 0 : src) * p.in_ld;
     const uint16_t* b = a + p.cols;   // SwiGLU: [gate | up]
+    // columns c (even) and c + 1, in the pairs of the other kernel
+    auto activated_at = [&](int64_t c) {
+      const bool two = c + 1 < p.cols;
+      return activated<kAct>(pair_of(bf16_at(a, c), two ? bf16_at(a, c + 1) : 0.f),
+                             kAct == FP8GMM_ACT_SWIGLU ? pair_of(bf16_at(b, c), two ? bf16_at(b, c + 1) : 0.f) : both(0.f));
+    };
     uint32_t top = 0;
     if (src >= 0)
-      for (int64_t c = threadIdx.x; c < p.cols; c += kLongThreads) {
-        const float v = activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f);
-        top = max(top, __float_as_uint(v) & 0x7FFFFFFFu);
+      for (int64_t c = 2 * threadIdx.x; c < p.cols; c += 2 * kLongThreads) {
+        const float2 v = split(activated_at(c));
+        top = max(top, max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu));
       }
     const RowScale s = row_scale(row_max(top, warp_max[turn]));
     if (threadIdx.x == 0) p.scales[r] = s.scale;
     const bool zero = s.pre == 0.f;
-    for (int64_t c = threadIdx.x; c < p.cols; c += kLongThreads) {
-      uint32_t q = 0;
-      if (!zero) q = code_of<kAct>(activated<kAct>(bf16_at(a, c), kAct == FP8GMM_ACT_SWIGLU ? bf16_at(b, c) : 0.f), s);
-      p.codes[r * p.codes_ld + c] = static_cast<int8_t>(q & 0xFFu);
+    for (int64_t c = 2 * threadIdx.x; c < p.cols; c += 2 * kLongThreads) {
+      const uint2 q = zero ? make_uint2(0u, 0u) : codes_of<kAct>(activated_at(c), s);
+      int8_t* out = p.codes + r * p.codes_ld + c;
+      out[0] = static_cast<int8_t>(q.x & 0xFFu);
+      if (c + 1 < p.cols) out[1] = static_cast<int8_t>(q.y & 0xFFu);
     }
   }
 }
@@ -207,13 +262,15 @@ void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
   const int64_t vecs = p.cols / 8;
   const bool aligned = p.cols % 8 == 0 && p.codes_ld % 8 == 0 && p.in_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
   if (aligned && vecs <= kMaxThreads * kMaxVecs && p.rows <= INT32_MAX) {
-    // Four vectors per thread keep more bytes in flight (measured against two: 32768 rows of 4096 69 / 81 us, behind SwiGLU
-    // 14336 wide 384 / 434 us = 6.1 TB/s); two answer sooner where all rows run at once, and fill a warp with a short row
-    // (100000 rows of 272: 29 / 37 us).  Short rows share a block, since starting a block takes about 1 ns of the GPU's
-    // time (one row per block: 262144 rows of 1024 took 272 us, now 126).
+    // Four vectors per thread keep more bytes in flight (measured against two: 32768 rows of 4096 61 / 71 us, 262144 rows of 1024
+    // 117 / 138); two answer sooner where all rows run at once (300 rows of 4096 2.5 / 2.9 us), and fill a warp with a short row
+    // (100000 rows of 272: 25 / 32 us).  Short rows share a block, since starting a block takes about 1 ns of the GPU's time
+    // (one row per block: 262144 rows of 1024 took 271 us, 100000 of 272 105), but no more than that needs: blocks of 128 threads
+    // against 256, 32768 rows of 4096 60 / 61.5, behind SwiGLU 98 / 103, 1200 behind GELU 5.1 / 5.4, 100000 rows of 272 29 / 25.
     const int per = vecs <= 64 || (vecs <= 2 * kMaxThreads && p.rows <= 4 * sm_count()) ? 2 : 4;
     const int threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
-    const int rows_per_block = threads < 256 ? 256 / threads : 1;
+    const int block_threads = vecs <= 64 ? 256 : 128;
+    const int rows_per_block = threads < block_threads ? block_threads / threads : 1;
     const dim3 block(threads, rows_per_block);
     const unsigned int grid = static_cast<unsigned int>((p.rows + rows_per_block - 1) / rows_per_block);
     if (per == 2) quantize_rows_kernel<kAct, 2><<<grid, block, 0, s>>>(p);
