@@ -699,7 +699,8 @@ def quantize_rows_int8(x, indices=None, top_k=1, activation=None, codes=None, sc
 
     x: (..., cols) bf16, rows contiguous.  ``indices`` (CUDA int32, from ``routing.indices_and_bins``): row r is taken
     from ``x[indices[r] // top_k]``, the gather of an MoE block.  ``activation``: "gelu" (tanh form) or "swiglu" (x is
-    [gate | up], the codes half as wide) is applied first, in fp32.  A row of zeros has scale 0; a row with an infinity
+    [gate | up], the codes half as wide) is applied first, in fp32 (``v`` within a few units in the last place; the codes are
+    the correctly rounded quotients of that ``v``).  A row of zeros has scale 0; a row with an infinity
     or a NaN has codes 0 and scale NaN, so every product of it is NaN.  Weights (G, N, K) give codes of that shape and
     scales (G, N).  ``codes`` / ``scales``: written in place when given.
     """

@@ -3,17 +3,19 @@
 //
 //   v[r, :] = act(x[src(r), :]),  top = max_k |v[r, k]|,  scale[r] = top / 127,  code[r, k] = round_half_even(127 v[r, k] / top)
 //
-// The code is the correctly rounded quotient, not v * (1 / scale): with bf16 inputs 127 v / top is exactly half-way between
-// two codes quite often (v = top / 2 already is), and a reciprocal's error would send such values either way.  With t = 127 v
-// (exact: 8 + 7 significant bits), y = t * (1 / top) is off by less than 2 ulp and one residual step, y + (t - y top) / top
-// with a fused multiply-add for the exact residual, gives the representable half-way values exactly; any other quotient of a
-// 15-bit by an 8-bit number is further from half-way than fp32's rounding.  Both are scaled by a power of two first, so that
-// neither the reciprocal nor the product leaves fp32's range.
+// The code is the correctly rounded quotient of the fp32 number v, not v * (1 / scale): with bf16 inputs 127 v / top is exactly
+// half-way between two codes quite often (v = top / 2 already is), and a reciprocal's error would send such values either way.
+// Without an activation t = 127 v is exact (8 + 7 significant bits), y = t * (1 / top) is off by less than 2 ulp and one residual
+// step, y + (t - y top) / top with a fused multiply-add for the exact residual, gives the representable half-way values exactly;
+// any other quotient of a 15-bit by an 8-bit number is further from half-way than fp32's rounding.  Behind an activation there are
+// half-way quotients too (GELU returns its argument above 6), and v has 24 bits: see codes_of.  t and top are scaled by a power of
+// two first, so that neither the reciprocal nor the product leaves fp32's range.
 // A row of zeros has scale 0 and codes 0.  A row that holds an infinity or a NaN has scale NaN and codes 0: all its products
 // come out NaN, no other row's do.
 //
 // Two kernels.  quantize_rows_kernel: a block for one row or several short ones, the row in registers between the maximum and the
-// codes, so it is read once; 16-byte loads, 8-byte stores.  quantize_long_rows_kernel: rows that are too long for that, or not
+// codes, so it is read once; 16-byte loads, 8-byte stores; 64 registers behind an activation (with 40 the values spill: 131 us
+// instead of 116 for 32768 rows of 4096 behind SwiGLU).  quantize_long_rows_kernel: rows that are too long for that, or not
 // aligned to 16 bytes, are walked twice (the second time out of L2 or L1).
 #include "int8.cuh"
 
@@ -41,9 +43,8 @@ struct QuantRowsParams {
 __device__ __forceinline__ float bf16_at(const uint16_t* p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
 
 // Two floats in a register pair: one instruction for both where there is a packed form, each rounded as on its own.  The kernel is
-// bound by its instructions as much as by HBM: 32768 rows of 4096 took 69 us with single ones and 61.5 with these; behind GELU 89
-// and 77, behind SwiGLU 106 and 102.  (Behind an activation the special function unit is next, two operations an element at an
-// eighth of the rate; one reciprocal shared by two elements saved a quarter of them and cost more in the test for its range: 93.)
+// bound by its instructions as much as by HBM: 32768 rows of 4096 took 69 us with single ones and 61.5 with these.  (Behind an
+// activation the special function unit is next, two operations an element at an eighth of the rate.)
 struct Pair {
   uint64_t v;
 };
@@ -84,41 +85,53 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-// a / (1 + 2^p) from the hardware's exp2 and reciprocal, a few ulp (the rounding of exp2's argument, |p| 2^-24, is larger from
-// |p| = 4 on).  Both instructions flush subnormal numbers, so the quotient is taken 16 times as large, 16 / (1 + e) =
-// 1 / (1/16 + 2^(p - 4)): it then stays normal for every e = 2^p in fp32's range.  An exp that overflows gives 0.
-// The two share a reciprocal, 1 / d = d' / (d d'), unless d d' leaves the range in which that stays normal: the special function
-// unit, at an eighth of the others' rate, is what limits this kernel behind an activation.
-constexpr float kLog2E = 1.44269504f;
-__device__ __forceinline__ Pair over_one_plus_exp2(Pair a, Pair powers_minus_4) {
-  const float2 p = split(powers_minus_4);
-  const float2 d = split(add2(pair_of(exp2_approx(p.x), exp2_approx(p.y)), both(0.0625f)));
-  const Pair inv = pair_of(rcp_approx(d.x), rcp_approx(d.y));
-  return mul2(mul2(a, both(0.0625f)), inv);
+// v = a / (1 + e), e = 2^p: exp2 and reciprocal of the special function unit (relative errors 2^-22 and 2^-23), then one
+// residual step that takes the quotient to the rounding of v itself.  The sum is taken half as large: the reciprocal flushes
+// subnormal results, and this keeps it normal up to p = 127; beyond, e is at most fp32's largest number and v comes out as 0.
+// Against 64 bits 25 codes of 2 * 10^8 differ behind SiLU and 21 behind GELU (normal rows with a few large values), as many as
+// with IEEE division and expf; without the residual steps here and in codes_of it was 772 behind GELU.  32768 rows of 4096 take
+// 93 us behind GELU and 116 behind SwiGLU, 75 and 97 without those steps.  Tried: 2^p from a polynomial and the sum in two floats,
+// 21 and 21 codes, but 141 and 155 us.
+constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even, into the low bits
+__device__ __forceinline__ Pair exp2_approx(Pair p) {
+  const float2 x = split(p);
+  return pair_of(exp2_approx(x.x), exp2_approx(x.y));
+}
+__device__ __forceinline__ Pair over_one_plus(Pair a, Pair e) {
+  const float2 es = split(e);   // the smaller number, also of a NaN: those of `a` come back through the product with it
+  const Pair minus_d = fma2(pair_of(fminf(es.x, 3.4028235e38f), fminf(es.y, 3.4028235e38f)), both(-0.5f), both(-0.5f));
+  const float2 ds = split(minus_d);
+  const Pair inv = pair_of(rcp_approx(-ds.x), rcp_approx(-ds.y)), half = mul2(a, both(0.5f)), v = mul2(half, inv);
+  return fma2(fma2(v, minus_d, half), inv, v);
 }
 template <int kAct>
 __device__ __forceinline__ Pair activated(Pair a, Pair b) {
-  if constexpr (kAct == FP8GMM_ACT_SWIGLU) return mul2(over_one_plus_exp2(a, fma2(a, both(-kLog2E), both(-4.f))), b);
+  if constexpr (kAct == FP8GMM_ACT_SWIGLU) {
+    // p = -a log2(e): log2(e) in 16 bits, whose product with a bf16 number is exact, and 2^x = 1 + x ln 2 for the rest
+    constexpr float kHigh = 0x1.7154p0f, kRest = 7.0526075e-06f * 0.69314718f;
+    const Pair e = exp2_approx(mul2(a, both(-kHigh)));
+    return mul2(over_one_plus(a, fma2(e, mul2(a, both(-kRest)), e)), b);
+  }
   if constexpr (kAct == FP8GMM_ACT_GELU) {
     // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), without the cancellation of 1 + tanh u at
-    // negative u; the power of two is -2u log2(e) = a (c + 0.044715 c a^2)
-    constexpr float kC = -2.f * 0.79788456f * kLog2E;
-    return over_one_plus_exp2(a, fma2(a, fma2(mul2(a, a), both(0.044715f * kC), both(kC)), both(-4.f)));
+    // negative u; the power of two is -2u log2(e) = a (k + 0.044715 k a^2)
+    constexpr float k = static_cast<float>(-2 * 0.79788456 * 1.4426950408889634), k3 = static_cast<float>(-2 * 0.79788456 * 1.4426950408889634 * 0.044715);
+    return over_one_plus(a, exp2_approx(mul2(a, fma2(mul2(a, a), both(k3), both(k)))));
   }
   return a;
 }
 
-// Factors of one row: t = v * pre, y = t * inv, residual against `top`.
+// Factors of one row: t = v * pre, y = t * inv, residuals against `top`; a residual of `limit` or more calls for a closer look.
 struct RowScale {
-  float pre, inv, top, scale;
+  float pre, inv, top, limit, scale;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
   RowScale s;
-  const float top = __uint_as_float(top_bits);
+  const float top = __uint_as_float(top_bits), inf = __uint_as_float(0x7F800000u);
   if (top_bits >= 0x7F800000u) {          // infinity or NaN
-    s = {0.f, 0.f, 0.f, __uint_as_float(0x7FC00000u)};
+    s = {0.f, 0.f, 0.f, inf, __uint_as_float(0x7FC00000u)};
   } else if (top_bits == 0u) {
-    s = {0.f, 0.f, 0.f, 0.f};
+    s = {0.f, 0.f, 0.f, inf, 0.f};
   } else {
     int e = 127 - static_cast<int>(top_bits >> 23);   // 2^e * top is in [1, 2) for normal numbers
     e = max(-126, min(e, 120));
@@ -126,30 +139,46 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
     s.pre = 127.f * two_e;
     s.top = top * two_e;
     s.inv = __frcp_rn(s.top);
+    s.limit = 0.49999f * s.top;
     s.scale = __fdiv_rn(top, 127.f);
   }
   return s;
-}
-// The codes in the low bytes: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.  Behind
-// an activation there are no exact ties to respect (v itself is rounded), and the quotient is not corrected.
-template <int kAct>
-__device__ __forceinline__ uint2 codes_of(Pair v, const RowScale& s) {
-  const Pair magic = both(12582912.f), t = mul2(v, both(s.pre));
-  Pair y;
-  if constexpr (kAct != FP8GMM_ACT_NONE) {
-    y = fma2(t, both(s.inv), magic);
-  } else {
-    y = mul2(t, both(s.inv));
-    y = add2(fma2(fma2(y, both(-s.top), t), both(s.inv), y), magic);
-  }
-  const float2 r = split(y);
-  return make_uint2(__float_as_uint(r.x), __float_as_uint(r.y));
 }
 // max(a, |b|), NaN if either is
 __device__ __forceinline__ float max_abs(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
   return r;
+}
+
+// The codes of a pair in the low bytes (kRound + code).  `worst` collects the largest residual |t - code top| behind an activation:
+// t is off by up to 2^-24 of 127.5 top there, so a residual below 0.49999 top proves the code to be the nearest integer.
+template <int kAct>
+__device__ __forceinline__ uint2 codes_of(Pair v, const RowScale& s, float& worst) {
+  const Pair t = mul2(v, both(s.pre));
+  float2 r;
+  if constexpr (kAct != FP8GMM_ACT_NONE) {
+    const Pair z = fma2(t, both(s.inv), both(kRound));
+    const float2 left = split(fma2(add2(z, both(-kRound)), both(-s.top), t));
+    worst = max_abs(max_abs(worst, left.x), left.y);
+    r = split(z);
+  } else {
+    const Pair y = mul2(t, both(s.inv));
+    r = split(add2(fma2(fma2(y, both(-s.top), t), both(s.inv), y), both(kRound)));
+  }
+  return make_uint2(__float_as_uint(r.x), __float_as_uint(r.y));
+}
+// The code of a value whose vector of eight holds a residual of `limit` or more (one in 6000), from the quotient in 64 bits: 127 v
+// has 31 bits and top 24, so its distance from half-way is 0 or far more than the quotient's rounding.
+__device__ __forceinline__ uint32_t exact_code(float v, float top) {
+  return static_cast<uint32_t>(__double2int_rn(__ddiv_rn(127.0 * static_cast<double>(v), static_cast<double>(top))));
+}
+__device__ __forceinline__ uint32_t exact_codes(Pair v, float top) {
+  const float2 x = split(v);
+  return (exact_code(x.x, top) & 0xFFu) | (exact_code(x.y, top) & 0xFFu) << 8;
+}
+__device__ __noinline__ uint2 exact_codes(Pair a, Pair b, Pair c, Pair d, float top) {
+  return make_uint2(exact_codes(a, top) | exact_codes(b, top) << 16, exact_codes(c, top) | exact_codes(d, top) << 16);
 }
 
 // Maximum over the threads of one row (blockDim.x of them, whole warps) of bits of non-negative floats (ordered like them, NaN
@@ -175,7 +204,7 @@ __device__ __forceinline__ int64_t source_row(const QuantRowsParams& p, int64_t 
 }
 
 template <int kAct, int kVecs>
-__global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_ACT_SWIGLU ? 2 : 3) quantize_rows_kernel(const QuantRowsParams p) {
+__global__ void __launch_bounds__(kMaxThreads, kAct != FP8GMM_ACT_NONE ? 2 : kVecs == 2 ? 4 : 3) quantize_rows_kernel(const QuantRowsParams p) {
   __shared__ uint32_t warp_max[kMaxThreads / 32];
   let_dependents_start();
   const int64_t r = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -205,7 +234,8 @@ __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_A
       top = max_abs(max_abs(top, x.x), x.y);
     }
   }
-  const RowScale s = row_scale(row_max(__float_as_uint(top), warp_max + threadIdx.y * (blockDim.x >> 5)));
+  const uint32_t top_bits = row_max(__float_as_uint(top), warp_max + threadIdx.y * (blockDim.x >> 5));
+  const RowScale s = row_scale(top_bits);
   if (!live) return;
   if (threadIdx.x == 0) p.scales[r] = s.scale;
   const bool zero = s.pre == 0.f;
@@ -215,12 +245,13 @@ __global__ void __launch_bounds__(kMaxThreads, kVecs == 2 ? 4 : kAct == FP8GMM_A
     const int c = threadIdx.x + u * blockDim.x;
     if (c >= vecs) break;
     uint32_t q[2];
+    float worst = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint2 a2 = codes_of<kAct>(v[u][2 * h], s), b2 = codes_of<kAct>(v[u][2 * h + 1], s);
+      const uint2 a2 = codes_of<kAct>(v[u][2 * h], s, worst), b2 = codes_of<kAct>(v[u][2 * h + 1], s, worst);
       q[h] = zero ? 0u : __byte_perm(__byte_perm(a2.x, a2.y, 0x0040), __byte_perm(b2.x, b2.y, 0x0040), 0x5410);
     }
-    out[c] = make_uint2(q[0], q[1]);
+    out[c] = kAct != FP8GMM_ACT_NONE && worst >= s.limit ? exact_codes(v[u][0], v[u][1], v[u][2], v[u][3], __uint_as_float(top_bits)) : make_uint2(q[0], q[1]);
   }
 }
 
@@ -245,11 +276,16 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
         const float2 v = split(activated_at(c));
         top = max(top, max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu));
       }
-    const RowScale s = row_scale(row_max(top, warp_max[turn]));
+    top = row_max(top, warp_max[turn]);
+    const RowScale s = row_scale(top);
     if (threadIdx.x == 0) p.scales[r] = s.scale;
     const bool zero = s.pre == 0.f;
     for (int64_t c = 2 * threadIdx.x; c < p.cols; c += 2 * kLongThreads) {
-      const uint2 q = zero ? make_uint2(0u, 0u) : codes_of<kAct>(activated_at(c), s);
+      const Pair v = activated_at(c);
+      float worst = 0.f;
+      uint2 q = codes_of<kAct>(v, s, worst);
+      if (kAct != FP8GMM_ACT_NONE && worst >= s.limit) q = make_uint2(exact_code(split(v).x, __uint_as_float(top)), exact_code(split(v).y, __uint_as_float(top)));
+      if (zero) q = make_uint2(0u, 0u);
       int8_t* out = p.codes + r * p.codes_ld + c;
       out[0] = static_cast<int8_t>(q.x & 0xFFu);
       if (c + 1 < p.cols) out[1] = static_cast<int8_t>(q.y & 0xFFu);
@@ -266,7 +302,7 @@ void launch_rows(const QuantRowsParams& p, cudaStream_t s) {
     // 117 / 138); two answer sooner where all rows run at once (300 rows of 4096 2.5 / 2.9 us), and fill a warp with a short row
     // (100000 rows of 272: 25 / 32 us).  Short rows share a block, since starting a block takes about 1 ns of the GPU's time
     // (one row per block: 262144 rows of 1024 took 271 us, 100000 of 272 105), but no more than that needs: blocks of 128 threads
-    // against 256, 32768 rows of 4096 60 / 61.5, behind SwiGLU 98 / 103, 1200 behind GELU 5.1 / 5.4, 100000 rows of 272 29 / 25.
+    // against 256, 32768 rows of 4096 60 / 61.5, behind SwiGLU 116 / 121, 1200 behind GELU 6.0 / 6.5, 100000 rows of 272 29 / 25.
     const int per = vecs <= 64 || (vecs <= 2 * kMaxThreads && p.rows <= 4 * sm_count()) ? 2 : 4;
     const int threads = static_cast<int>(((vecs + per - 1) / per + 31) / 32 * 32);
     const int block_threads = vecs <= 64 ? 256 : 128;

@@ -408,7 +408,8 @@ int fp8gmm_moe_rowdot(const void* grad, const void* x, const int32_t* inverse, i
  * Rows of bf16 -> int8 codes and one fp32 scale per row:
  *   v = act(in[src(r), :]), top = max|v|, scales[r] = top / 127, codes[r, k] = round_half_even(127 * v[k] / top)
  * with src(r) = r, or indices[r] / top_k (the permutation fp8gmm_moe_sort writes: the gather of an MoE block, fused).
- * activation: FP8GMM_ACT_NONE, _GELU (tanh form), or _SWIGLU (a row of `in` is then [gate | up], 2 * cols wide).
+ * activation: FP8GMM_ACT_NONE, _GELU (tanh form), or _SWIGLU (a row of `in` is then [gate | up], 2 * cols wide); it is
+ * applied in fp32 (v within a few units in the last place), the quotient of the fp32 v and top is rounded correctly.
  * A row of zeros gets scale 0; a row with an infinity or a NaN gets codes 0 and scale NaN.  An index that names no row of
  * `in` gives codes 0 and scale 0 and is reported through the device status word.
  * Weights (G x N x K) are quantised per output channel by the same call, as G * N rows of K columns.
