@@ -947,15 +947,22 @@ def delayed_scaling_update(amax_history, scale, scale_inv, fp8_max, margin=0, al
           "delayed_scaling_update")
 
 
+# Bits of the device status word that say that a bounded wait ran out; the others report input that a kernel left out
+# (fp8gmm_status_bits).
+STATUS_WAITS = 0xF | 0x100
+
+
 def device_status():
-    """Synchronise the current stream and raise if a kernel reported a bounded wait that ran out."""
+    """Synchronise the current stream, clear the status word and raise if a kernel reported in it a bounded wait that ran out
+    (outputs undefined) or input that it left out (an index that names no row or expert, group sizes that do not fit)."""
     check(lib.fp8gmm_device_status(_stream()), "device_status")
 
 
 class StatusWatch:
     """Non-blocking view of the device status word for training loops: ``record()`` enqueues a copy of the word
     into page-locked host memory on the current stream, ``check()`` raises if a copy that has already landed shows
-    that a bounded wait ran out (the outputs of that launch, and everything computed from them, are undefined)."""
+    that a bounded wait ran out (the outputs of that launch, and everything computed from them, are undefined) or, unless
+    ``waits_only``, that a kernel left out bad input.  The word keeps its bits until ``device_status()``."""
 
     def __init__(self):
         self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
@@ -963,9 +970,13 @@ class StatusWatch:
     def record(self):
         check(lib.fp8gmm_device_status_async(self.host.data_ptr(), _stream()), "device_status_async")
 
-    def check(self):
+    def check(self, waits_only=False):
         code = int(self.host[0])
-        if code != 0:
+        if code & STATUS_WAITS:
             raise RuntimeError(
                 f"fp8_gmm_b200: a kernel gave up on a bounded wait in an earlier step (status 0x{code:x}: a peer was "
                 "late or a copy never arrived); results since then are undefined")
+        if code != 0 and not waits_only:
+            raise RuntimeError(
+                f"fp8_gmm_b200: a kernel left out bad input in an earlier step (status 0x{code:x}: indices that name no row or "
+                "expert, or group sizes that do not fit the rows); its other results stand")

@@ -31,7 +31,7 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kMaxGroups = 512;
-constexpr int kStatusBadSizes = 0x400;   // group sizes that are negative or reach behind the last row
+constexpr int kStatusBadSizes = FP8GMM_STATUS_BAD_SIZES;   // group sizes that are negative or reach behind the last row
 constexpr int kThreads = 320;            // TMA producer warp, MMA warp, two groups of four epilogue warps
 constexpr int kChannels = 128;           // channels of one CTA's half of the MMA
 constexpr int kAtomK = 128;              // bytes of contraction in one box: a 128-byte swizzle atom

@@ -25,7 +25,7 @@ namespace {
 constexpr int kLongThreads = 256;
 constexpr int kMaxThreads = 512;
 constexpr int kMaxVecs = 4;              // 8-element vectors a thread holds: rows of up to 512 * 4 * 8 = 16384 elements
-constexpr int kStatusBadIndex = 0x200;   // as in routing.cu: an index that names no row
+constexpr int kStatusBadIndex = FP8GMM_STATUS_BAD_INDEX;
 
 struct QuantRowsParams {
   const uint16_t* in;

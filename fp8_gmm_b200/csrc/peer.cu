@@ -20,7 +20,7 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kMaxPeers = 64;
-constexpr int kStatusPeerTimeout = 0x100;
+constexpr int kStatusPeerTimeout = FP8GMM_STATUS_PEER_WAIT;
 
 struct SignalParams {
   uint32_t* flags[kMaxPeers];

@@ -19,7 +19,7 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kSortThreads = 1024;
-constexpr int kStatusBadExpertId = 0x200;   // an expert id outside [0, num_experts), or a row index it left unset
+constexpr int kStatusBadExpertId = FP8GMM_STATUS_BAD_INDEX;   // an expert id outside [0, num_experts), or a row index it left unset
 
 // Number of entries equal to `expert`, one CTA per expert.
 __global__ void __launch_bounds__(kSortThreads) moe_count_kernel(const int32_t* __restrict__ ids, int64_t n, int num_experts,

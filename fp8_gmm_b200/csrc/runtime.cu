@@ -124,7 +124,11 @@ int fp8gmm_device_status(void* stream) {
   if (host != 0) {
     const int zero = 0;
     FP8GMM_CHECK_CUDA(cudaMemcpy(word, &zero, sizeof(int), cudaMemcpyHostToDevice));
-    fp8gmm::set_error("a kernel gave up on a bounded wait (code 0x%x)", host);
+    const bool waits = (host & (FP8GMM_STATUS_GEMM_WAIT | FP8GMM_STATUS_PEER_WAIT)) != 0;
+    fp8gmm::set_error("%s%s%s%s (code 0x%x)", waits ? "a kernel gave up on a bounded wait" : "a kernel left out bad input",
+                      waits && (host & (FP8GMM_STATUS_BAD_INDEX | FP8GMM_STATUS_BAD_SIZES)) ? ", and one left out bad input" : "",
+                      host & FP8GMM_STATUS_BAD_INDEX ? ": an index that names no row or expert" : "",
+                      host & FP8GMM_STATUS_BAD_SIZES ? ": group sizes that do not fit the rows" : "", host);
     return FP8GMM_DEVICE_TIMEOUT;
   }
   return FP8GMM_OK;

@@ -906,7 +906,7 @@ def forward(module, input, group_sizes, is_first_microbatch, num_chunks):
     ectx = EpContext.setup(input.device, module.group)
     if not ectx.failed:
         try:
-            ectx.status.check()
+            ectx.status.check(waits_only=True)   # bad input to another call on this device is not the exchange's affair
         except RuntimeError:
             ectx.failed = True     # no further pushes into buffers whose state is unknown
             raise

@@ -32,8 +32,18 @@ typedef enum {
   FP8GMM_INVALID_ARGUMENT = 1, /* shape / alignment / NULL-pointer contract violated; nothing was launched */
   FP8GMM_CUDA_ERROR = 2,       /* a CUDA runtime or driver call failed; see fp8gmm_last_error() */
   FP8GMM_UNSUPPORTED = 3,      /* device is not sm_100, or a size exceeds a documented limit */
-  FP8GMM_DEVICE_TIMEOUT = 4    /* reported by fp8gmm_device_status(): a bounded wait in a kernel ran out */
+  FP8GMM_DEVICE_TIMEOUT = 4    /* reported by fp8gmm_device_status(): a bounded wait in a kernel ran out, or a kernel left out
+                                  input that it cannot use; the message says which */
 } fp8gmm_status;
+
+/* Bits of the device status word.  After a wait that ran out the outputs of that launch are undefined; bad input is left
+ * out as the entry point describes, and every other output is as it should be. */
+typedef enum {
+  FP8GMM_STATUS_GEMM_WAIT = 0xF,   /* a role of a persistent GEMM gave up on an mbarrier (one bit per kind of wait) */
+  FP8GMM_STATUS_PEER_WAIT = 0x100, /* fp8gmm_peer_wait gave up on a peer */
+  FP8GMM_STATUS_BAD_INDEX = 0x200, /* an expert id, or an index that names no row (fp8gmm_moe_*, fp8gmm_quantize_rows_int8) */
+  FP8GMM_STATUS_BAD_SIZES = 0x400  /* group sizes on the device that do not fit the rows (fp8gmm_int8_grouped_gemm) */
+} fp8gmm_status_bits;
 
 typedef enum { FP8GMM_E4M3 = 0, FP8GMM_E5M2 = 1 } fp8gmm_format;
 
@@ -48,16 +58,16 @@ const char* fp8gmm_last_error(void);
 /*
  * Synchronises `stream`, then reads and clears the device-side status word of the current device.
  * Returns FP8GMM_OK, FP8GMM_DEVICE_TIMEOUT (a kernel gave up on a bounded wait and returned without
- * finishing; outputs of that launch are undefined) or FP8GMM_CUDA_ERROR.  Meant for tests and
- * debugging; the hot path does not call it.
+ * finishing, so that outputs of that launch are undefined, or left out bad input: fp8gmm_status_bits; the message
+ * names the word) or FP8GMM_CUDA_ERROR.  Meant for tests and debugging; the hot path does not call it.
  */
 int fp8gmm_device_status(void* stream);
 
 /*
  * Enqueues on `stream` a copy of the device-side status word into `host_word` (page-locked host memory owned by
  * the caller) without synchronising and without clearing the word.  A training loop calls it at the end of a step
- * and looks at `*host_word` when it starts the next one: non-zero means a bounded wait ran out in some earlier
- * launch, whose outputs are then undefined.
+ * and looks at `*host_word` when it starts the next one: FP8GMM_STATUS_GEMM_WAIT and _PEER_WAIT mean that a bounded
+ * wait ran out in some earlier launch, whose outputs are then undefined; the other bits that input was left out.
  */
 int fp8gmm_device_status_async(int* host_word, void* stream);
 
