@@ -758,7 +758,7 @@ def _int8_gemm_args(device, rows, k, b, group_sizes, b_scales, c, name):
 def int8_gmm(a, b, group_sizes, a_scales, b_scales, c=None):
     """Grouped product of int8 codes, ``c[r] = bf16((a[r] . b[g]^T) * a_scales[r] * b_scales[g])`` for the rows r of group g.
 
-    a: (rows, K) int8, b: (G, N, K) int8, a_scales (rows,) and b_scales (G, N) fp32.  The 32-bit integer sums are exact.
+    a: (rows, K) int8, b: (G, N, K) int8, a_scales (rows,) and b_scales (G, N) fp32 of any size.  The 32-bit integer sums are exact.
     ``group_sizes``: one size per group, a CPU int64 tensor or a sequence as everywhere in this package (they sum to
     the rows), or a CUDA int64 tensor that is read when the kernel runs: then nothing waits for the host, the call can
     be captured into a graph and replayed with other sizes, and rows behind the last group are left as they are.

@@ -4,7 +4,7 @@
 //
 // The sum is an exact 32-bit integer (|a|, |b| <= 128 and K < 2^17), so every tile shape and every split of the contraction
 // gives the same bits; the conversion to float, the product of the scales, the product with them and the final bf16 are the
-// only roundings.
+// only roundings.  Where the product of the two scales leaves fp32's normal range the three factors are multiplied in 64 bits.
 //
 // The operands are swapped against gemm_sm100.cu: output channels are the M dimension of the MMA (TMEM lanes), rows the N
 // dimension (TMEM columns).  A group of any number of rows then costs an MMA only as wide as its rows, and a warp's 32 lanes
@@ -17,7 +17,7 @@
 //     box in shared memory and written as 256-byte runs; two groups of four warps take the chunks in turns.  This bounds products
 //     with short contractions (8 x 4096 rows, 28672 channels, 512 contraction bytes, 1.9 GB written: 560 us; with one group that
 //     stored 2 bytes per lane into the box 1123, with two 787, with fragments and stmatrix 690, with the arrival that does not
-//     wait for the stores 599, with the rows' addresses carried along 560; HBM's floor is 308).  With 4096 contraction bytes it
+//     wait for the stores 599, with the rows' addresses carried along 560, with the look at the scales' sizes 570; HBM's floor is 308).  With 4096 contraction bytes it
 //     is hidden behind the MMAs.
 // Group sizes come from the host (parameter block) or are read on the device; either way every CTA builds the prefix sums of
 // rows and tiles in shared memory.  Waits on mbarriers are bounded as in gemm_sm100.cu.
@@ -37,6 +37,7 @@ constexpr int kChannels = 128;           // channels of one CTA's half of the MM
 constexpr int kAtomK = 128;              // bytes of contraction in one box: a 128-byte swizzle atom
 constexpr int kAtoms = 2;                // boxes along the contraction per stage
 constexpr int kBlockK = kAtoms * kAtomK;
+constexpr int kBoxPitch = kChannels * 2 + 16;   // bytes of a row in the epilogue's box: the 16-byte pieces of eight rows lie in different banks
 
 struct Int8GemmParams {
   CUtensorMap map_w;                     // weights (G*N, K), box of `channels` rows x 128 bytes
@@ -96,6 +97,19 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
 __device__ __forceinline__ float result(uint32_t acc, float row_scale, float channel_scale) {
   return __fmul_rn(__int2float_rn(static_cast<int>(acc)), __fmul_rn(row_scale, channel_scale));
 }
+// With any scales.  A product of scales that is subnormal has lost bits, one that overflows makes a NaN of a sum of 0, though the
+// result may be a normal number.  A tile whose scales are all `ordinary` takes `result`, which then gives the same bits.
+__device__ __forceinline__ float result_of_any(uint32_t sum, float row_scale, float channel_scale) {
+  const int acc = static_cast<int>(sum);
+  const float s = __fmul_rn(row_scale, channel_scale);
+  if (fabsf(s) >= 1.17549435e-38f && fabsf(s) <= 3.4028235e38f) return __fmul_rn(__int2float_rn(acc), s);
+  return __double2float_rn(static_cast<double>(acc) * static_cast<double>(row_scale) * static_cast<double>(channel_scale));
+}
+// The product of two such scales is 0 or a normal number.
+__device__ __forceinline__ bool ordinary(float scale) {
+  const float size = fabsf(scale);   // no branches: every tile starts with this
+  return (size <= 0x1p63f) & ((size >= 0x1p-62f) | (size == 0.f));
+}
 
 // Prefix sums of rows and tiles over the groups, by one warp.  Sizes read on the device are cut off at the last row.
 __device__ __forceinline__ void build_groups(const Int8GemmParams& p, int* row_start, int* tile_start, int lane) {
@@ -144,6 +158,33 @@ __device__ __forceinline__ void build_groups(const Int8GemmParams& p, int* row_s
   if (blockIdx.x == 0 && __any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.status, kStatusBadSizes);
 }
 
+// 32 rows of a warp's 32 channels through the scales into the box.  `row_scales`: of rows 2 (lane % 4) and the next, and every
+// eighth from there; `out`: where this lane's pieces of the transposed fragments go.
+template <bool kOrdinary>
+__device__ __forceinline__ void transpose_chunk(const uint32_t (&lo)[16], const uint32_t (&hi)[16], const float* row_scales, const float (&sb)[4], uint32_t out) {
+  auto value = [](uint32_t acc, float row_scale, float channel_scale) {
+    return kOrdinary ? result(acc, row_scale, channel_scale) : result_of_any(acc, row_scale, channel_scale);
+  };
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const float2 sa = *reinterpret_cast<const float2*>(row_scales + 8 * n);
+    store_transposed(out + 8 * n * kBoxPitch,
+                     pack_bf16x2(value(lo[4 * n], sa.x, sb[0]), value(lo[4 * n + 1], sa.y, sb[0])),
+                     pack_bf16x2(value(lo[4 * n + 2], sa.x, sb[1]), value(lo[4 * n + 3], sa.y, sb[1])),
+                     pack_bf16x2(value(hi[4 * n], sa.x, sb[2]), value(hi[4 * n + 1], sa.y, sb[2])),
+                     pack_bf16x2(value(hi[4 * n + 2], sa.x, sb[3]), value(hi[4 * n + 3], sa.y, sb[3])));
+  }
+}
+// Reads the fragments again: the loop over ordinary chunks keeps its code and registers.
+__device__ __noinline__ void transpose_chunk_of_any(uint32_t taddr, const float* row_scales, float s0, float s1, float s2, float s3, uint32_t out) {
+  uint32_t lo[16], hi[16];
+  tmem_ld_16x32(taddr, lo);
+  tmem_ld_16x32(taddr + (16u << 16), hi);
+  tc_wait_ld();
+  const float sb[4] = {s0, s1, s2, s3};
+  transpose_chunk<false>(lo, hi, row_scales, sb, out);
+}
+
 struct Tile {
   int group, row0, rows, n0;
 };
@@ -169,7 +210,6 @@ constexpr int kMaxRows = 256;                 // rows of the larger tile
 constexpr int kMaxStages = 12 / kAtoms;
 constexpr int kRingBytes = 6 * 32 * 1024;
 constexpr int kTmemCols = 512;
-constexpr int kBoxPitch = kChannels * 2 + 16; // bytes: the 16-byte pieces of eight rows lie in different banks
 constexpr int kBoxBytes = 32 * kBoxPitch;     // 32 rows x 128 channels of bf16
 constexpr int kStagingBytes = 2 * kBoxBytes;
 constexpr int kScaleBytes = 2 * kMaxRows * 4;
@@ -188,6 +228,16 @@ __device__ __forceinline__ int mma_width(int rows) { return (rows + 31) & ~31; }
 
 // Barrier of one group of epilogue warps.
 __device__ __forceinline__ void epilogue_barrier(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
+// The same, and whether `mine` is true in all threads of the group.
+__device__ __forceinline__ bool epilogue_barrier_all(int group, bool mine) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(all)
+      : "r"(mine ? 1u : 0u), "r"(1 + group)
+      : "memory");
+  return all != 0;
+}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_constant__ Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -397,10 +447,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
       const int n0 = t.n0 + rank * p.channels, n_end = min(n0 + p.channels, p.n);
       float* scales = scale_buf + acc * kMaxRows;
       scales[my_row] = next_sa;
+      const bool mine = ((my_row >= t.rows) | ordinary(next_sa)) & ordinary(sb[0]) & ordinary(sb[1]) & ordinary(sb[2]) & ordinary(sb[3]);
       fetch(tile + num_workers);
       if (lane == 0 && ok) ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 0x8, p.wait_ns);
       ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-      epilogue_barrier(group);
+      const bool all_ordinary = epilogue_barrier_all(group, mine);
       tc_fence_after();
       const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * kMaxRows) + (static_cast<uint32_t>(quad * 32) << 16);
 
@@ -413,15 +464,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
           tmem_ld_16x32(taddr + c0, lo);
           tmem_ld_16x32(taddr + c0 + (16u << 16), hi);
           tc_wait_ld();
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float2 sa = *reinterpret_cast<const float2*>(scales + c0 + 8 * n + 2 * (lane & 3));
-            store_transposed(box_out + 8 * n * kBoxPitch,
-                             pack_bf16x2(result(lo[4 * n], sa.x, sb[0]), result(lo[4 * n + 1], sa.y, sb[0])),
-                             pack_bf16x2(result(lo[4 * n + 2], sa.x, sb[1]), result(lo[4 * n + 3], sa.y, sb[1])),
-                             pack_bf16x2(result(hi[4 * n], sa.x, sb[2]), result(hi[4 * n + 1], sa.y, sb[2])),
-                             pack_bf16x2(result(hi[4 * n + 2], sa.x, sb[3]), result(hi[4 * n + 3], sa.y, sb[3])));
-          }
+          if (all_ordinary) transpose_chunk<true>(lo, hi, scales + c0 + 2 * (lane & 3), sb, box_out);
+          else transpose_chunk_of_any(taddr + c0, scales + c0 + 2 * (lane & 3), sb[0], sb[1], sb[2], sb[3], box_out);
         }
         epilogue_barrier(group);
         if (ok && writes) {

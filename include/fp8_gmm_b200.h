@@ -442,7 +442,8 @@ int fp8gmm_quantize_rows_int8(const fp8gmm_quantize_rows_args* args, void* strea
 
 /*
  * C[r, :] = bf16( (sum_k a[r, k] * b[g, :, k]) * a_scales[r] * b_scales[g, :] ) for every row r of group g; 32-bit integer
- * sums (exact: K < 131072).
+ * sums (exact: K < 131072).  The product of the two scales is rounded to fp32 where it is a normal number or 0; elsewhere
+ * the three factors are multiplied in 64 bits.
  *   a        int8 (rows x K), groups are consecutive row blocks; row pitch a_ld (a multiple of 16, 0 = K; one that is a
  *            multiple of 128 is read fastest)
  *   b        int8 (G x N x K) row-major
