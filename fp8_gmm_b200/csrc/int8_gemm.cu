@@ -371,6 +371,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) int8_ge
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
+      grid_dependency_wait();   // the limit of the waits below is for this kernel's own copies, not for the quantisation in front
       for (int tile = worker; tile < total_tiles; tile += num_workers) {
         const Tile t = decode_tile(p, row_start, tile_start, tile);
         const uint32_t idesc = idesc_i8(2 * kChannels, mma_width(t.rows));
