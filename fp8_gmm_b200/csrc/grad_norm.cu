@@ -247,6 +247,24 @@ __device__ __forceinline__ void clip_tile(const GradDesc& d, int64_t base, float
   else clip_tile<kIn, FP8GMM_F16>(d, base, coef);
 }
 
+__device__ __forceinline__ float load_one(const GradDesc& d, int64_t i) {
+  if (d.in_type == FP8GMM_F32) return static_cast<const float*>(d.in)[i];
+  if (d.in_type == FP8GMM_BF16) return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(d.in)[i]) << 16);
+  return __half2float(static_cast<const __half*>(d.in)[i]);
+}
+// With a factor below fp32's normal range, where it would lose bits that ordinary results need (a norm of 1e41 and a limit of 1:
+// elements of 1e38 become 1e-3): products in 64 bits, one element at a time.
+__device__ __noinline__ void clip_tile_by_double(const GradDesc& d, int64_t base, double c) {
+  for (int u = threadIdx.x; u < kTileElems; u += kThreads) {
+    const int64_t i = base + u;
+    if (i < 0 || i >= d.numel) continue;
+    const float v = static_cast<float>(static_cast<double>(load_one(d, i)) * c);
+    if (d.out_type == FP8GMM_F32) static_cast<float*>(d.out)[i] = v;
+    else if (d.out_type == FP8GMM_BF16) static_cast<__nv_bfloat16*>(d.out)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(d.out)[i] = __float2half_rn(v);
+  }
+}
+
 // One tile per CTA, from the last one to the first.
 template <int kMax>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_kernel(const __grid_constant__ GradArgs<kMax> args, const double* __restrict__ sums,
@@ -261,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_kernel(const __grid
   const double c = static_cast<double>(max_norm) / (n + 1e-6);
   const float coef = c >= 1.0 ? 1.f : static_cast<float>(c);  // a NaN norm keeps its NaN
   if (coef == 1.f && d.in == d.out) return;   // in place and within the limit: nothing changes
-  if (d.in_type == FP8GMM_BF16) clip_tile<FP8GMM_BF16>(d, base, coef);
+  if (c > 0.0 && c < 0x1p-126) clip_tile_by_double(d, base, c);
+  else if (d.in_type == FP8GMM_BF16) clip_tile<FP8GMM_BF16>(d, base, coef);
   else if (d.in_type == FP8GMM_F32) clip_tile<FP8GMM_F32>(d, base, coef);
   else clip_tile<FP8GMM_F16>(d, base, coef);
 }
