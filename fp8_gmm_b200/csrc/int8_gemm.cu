@@ -597,6 +597,7 @@ int int8_gemm_check(const fp8gmm_int8_gemm_args* a) {
   FP8GMM_CHECK_ARG(a->rows >= 0 && a->rows <= INT32_MAX - 1024, "int8_grouped_gemm: bad number of rows");
   FP8GMM_CHECK_ARG(a->num_groups == 0 || (a->m_sizes != nullptr) != (a->device_m_sizes != nullptr),
                    "int8_grouped_gemm: group sizes are given on the host or on the device, not both");
+  FP8GMM_CHECK_ARG(a->num_groups > 0 || a->rows == 0, "int8_grouped_gemm: %lld rows, but no groups", (long long)a->rows);
   int64_t sum = 0;
   for (int g = 0; a->m_sizes != nullptr && g < a->num_groups; ++g) {
     const int64_t m = a->m_sizes[g];
