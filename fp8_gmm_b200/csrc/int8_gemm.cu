@@ -563,7 +563,8 @@ double worker_time(int64_t groups, int64_t mean, int64_t tiles_n, int64_t tile_r
 // 3520 x 4096 with 300 rows 17.6 / 26.0, eight of 1536 x 4096 with 300 rows 19.0 / 26.5, with 1000 rows 46.4 / 41.6, eight of 8192 x 4096 with 300 rows
 // 89.4 / 92.6, with 2000 rows 458 / 387.  128 / 256 channels, 128 rows: two rows of 4096 x 14336 24.8 / 27.6, one expert of 256 x 1040 with 300
 // rows 7.3 / 7.9, of 768 x 4096 with 200 rows 9.8 / 10.1, three of 1536 x 4096 with 200 rows 11.4 / 10.6.  Over 405 shapes (1 to 8
-// experts, 64 to 2000 rows each, 256 to 8192 channels, 256 to 4096 bytes) the rule takes 0.6 % more than the best tile on average.
+// experts of equally many rows, 64 to 2000, 256 to 8192 channels, 256 to 4096 bytes) the rule takes 0.6 % more than the best tile on
+// average; with uneven groups it can miss the better one, by up to 18 % of the estimate above.
 // (Splitting the contraction of a partial wave's tiles between pairs, with sums handed on through L2, cost about 8 us a
 // tile: dropped.)
 struct TileShape {
